@@ -55,30 +55,30 @@ def _adamw(name, tensors, dtype, grads, bits, masters=False, width=0, layers=0):
 def listed():
     return [
         # serving: one token of each of 16 sequences, where the call itself is what counts
-        _token("recurrence, one token", 16, 1024, "bf16"),
+        _token("recurrence one token", 16, 1024, "bf16"),
         # serving: a long prompt, one sequence, its state kept for the tokens that follow
-        _recurrence("recurrence, long prompt", 1, 131072, 1024, "f16", train=False, state=True),
+        _recurrence("recurrence long prompt", 1, 131072, 1024, "f16", train=False, state=True),
         # training: a batch of ordinary lengths, forward and backward
-        _recurrence("recurrence, training", 8, 4096, 2048, "bf16"),
+        _recurrence("recurrence training", 8, 4096, 2048, "bf16"),
         # training in 32 bits on packed documents of ragged lengths, odd width, no output gate
-        _recurrence("recurrence, packed", 23, 331, 515, "f32", gate=False, packed=True, state=True),
+        _recurrence("recurrence packed", 23, 331, 515, "f32", gate=False, packed=True, state=True),
         # serving: the boundary between two blocks for a few tokens
-        _norms("norms, few tokens", 16, 1, 2048, "bf16", "bf16", train=False),
+        _norms("norms few tokens", 16, 1, 2048, "bf16", "bf16", train=False),
         # serving: a prompt, residual stream in 32 bits
-        _norms("norms, prompt", 1, 8192, 5120, "bf16", "f32", train=False),
+        _norms("norms prompt", 1, 8192, 5120, "bf16", "f32", train=False),
         # training: both norms, a gate computed from every token
-        _norms("norms, training", 8, 2048, 4096, "bf16", "bf16", gate="sigmoid"),
+        _norms("norms training", 8, 2048, 4096, "bf16", "bf16", gate="sigmoid"),
         # training in 32 bits: layer norms with biases, a gate for each sequence, nothing a power of two
-        _norms("norms, gate per sequence", 24, 513, 1000, "f32", "f32", post="layer", pre="layer", gate="linear",
+        _norms("norms gate per sequence", 24, 513, 1000, "f32", "f32", post="layer", pre="layer", gate="linear",
                per="sequence", bias=True),
         # the convolution layers of the benchmark: few tensors, some of them tiny
-        _adamw("adamw, conv layers", "conv", "f32", "f32", 32),
+        _adamw("adamw conv layers", "conv", "f32", "f32", 32),
         # a model's parameters in 32 bits
-        _adamw("adamw, 32-bit states", "blocks", "f32", "f32", 32, width=2048, layers=8),
+        _adamw("adamw 32-bit states", "blocks", "f32", "f32", 32, width=2048, layers=8),
         # 16-bit parameters with 32-bit masters, moments in 8 bits
-        _adamw("adamw, 8-bit, masters", "blocks", "bf16", "bf16", 8, masters=True, width=2048, layers=8),
+        _adamw("adamw 8-bit masters", "blocks", "bf16", "bf16", 8, masters=True, width=2048, layers=8),
         # 16-bit parameters alone, moments in 8 bits, tensors of odd sizes
-        _adamw("adamw, 8-bit, ragged", "ragged", "bf16", "f32", 8, width=1500, layers=60),
+        _adamw("adamw 8-bit ragged", "ragged", "bf16", "f32", 8, width=1500, layers=60),
     ]
 
 

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_size_t, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 # FBFFTCONV_LIB points at another build of the same library (tuning experiments)
@@ -43,6 +43,38 @@ class Desc(ctypes.Structure):
     ]
 
 
+FLOAT32 = 0
+BFLOAT16 = 1
+FLOAT16 = 2
+
+
+class AdamwTensor(ctypes.Structure):
+    """struct fbfftconv_adamw_tensor."""
+
+    _fields_ = [
+        ("param", c_void_p), ("master", c_void_p), ("grad", c_void_p), ("moment1", c_void_p), ("moment2", c_void_p),
+        ("scale1", c_void_p), ("scale2", c_void_p), ("count", c_int64), ("param_type", c_int32), ("grad_type", c_int32),
+    ]
+
+
+class AdamwOptions(ctypes.Structure):
+    """struct fbfftconv_adamw_options."""
+
+    _fields_ = [
+        ("beta1", c_double), ("beta2", c_double), ("eps", c_double), ("weight_decay", c_double),
+        ("steps", c_void_p), ("seed", c_uint32), ("device", c_int32),
+    ]
+
+
+def element_types() -> dict:
+    """The element types of the sequence-model operators, by torch type."""
+    global _types
+    if _types is None:
+        import torch
+        _types = {torch.float32: FLOAT32, torch.bfloat16: BFLOAT16, torch.float16: FLOAT16}
+    return _types
+
+
 class FbfftconvError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"fbfftconv status {status}: {message}")
@@ -50,6 +82,7 @@ class FbfftconvError(RuntimeError):
 
 
 _lib = None
+_types = None
 
 _SIGNATURES = {
     "fbfftconv_create": (c_int, [POINTER(Desc), POINTER(c_void_p)]),
@@ -93,6 +126,10 @@ _SIGNATURES = {
     "fbfftconv_update_output_bias": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
     "fbfftconv_acc_grad_parameters_bias": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p]),
     "fbfftconv_acc_grad_parameters_bias_noalloc": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p]),
+    "fbfftconv_adamw_create": (c_int, [POINTER(AdamwTensor), c_int, POINTER(AdamwOptions), POINTER(c_void_p)]),
+    "fbfftconv_adamw_destroy": (c_int, [c_void_p]),
+    "fbfftconv_adamw_set_gradients": (c_int, [c_void_p, POINTER(c_void_p), c_int]),
+    "fbfftconv_adamw_step": (c_int, [c_void_p, c_double, c_float, c_void_p, c_void_p]),
     "fbfftconv_profile_enable": (c_int, [c_void_p, c_int]),
     "fbfftconv_profile_reset": (c_int, [c_void_p]),
     "fbfftconv_profile_read": (c_int, [c_void_p, c_int, c_int, POINTER(ctypes.c_double), POINTER(c_int)]),

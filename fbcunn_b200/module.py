@@ -211,6 +211,11 @@ class SpatialConvolutionFBFFT:
             1.0 if scale is None else float(scale), _stream(self.device)))
         return self.gradInput
 
+    def parameters(self):
+        """nn.Module:parameters(): the learned tensors and their gradients."""
+        pairs = [(p, g) for p, g in ((self.weight, self.gradWeight), (self.bias, self.gradBias)) if p is not None]
+        return [p for p, _ in pairs], [g for _, g in pairs]
+
     def zeroGradParameters(self):
         self.gradWeight.zero_()
         self.gradBias.zero_()

@@ -177,6 +177,8 @@ class SpatialConvolution:
         self.gradInput = self.bestModuleInst.backward(input, gradOutput, scale)
         return self.gradInput
 
+    parameters = SpatialConvolutionFBFFT.parameters
+
     def zeroGradParameters(self):
         self.gradWeight.zero_()
         self.gradBias.zero_()

@@ -310,6 +310,53 @@ int fbfftconv_acc_grad_parameters_bias_noalloc(const float* grad_output, float* 
                                                int planes, int h, int w, float scale,
                                                int accumulate, fbfftconv_stream stream);
 
+/* ---- element types of the operators below -------------------------------------------------
+ * Values are computed in fp32 and rounded to nearest once, where they are stored. */
+enum { FBFFTCONV_FLOAT32 = 0, FBFFTCONV_BFLOAT16 = 1, FBFFTCONV_FLOAT16 = 2 };
+
+/* ---- AdamW over many tensors ----------------------------------------------------------------
+ * The step that consumes what accGradParameters leaves, for every tensor of a model in one launch:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,  g = grad_scale * grad
+ *   p = p (1 - lr weight_decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps)
+ * with t the number of this step, counted on the device, so that a captured step counts its replays.
+ *
+ * The moments of a tensor are fp32 (scale1 and scale2 null; moment2 holds v), or e4m3 codes with an fp32 scale for
+ * every 256 elements, counted from the tensor's first (moment2 then holds sqrt(v); a value is code * scale; scales for
+ * ceil(count / 256) blocks each).  Codes are rounded up or down at random in proportion to what is cut off, by a hash
+ * of seed, step, the tensor's place in the list and the element's in the tensor: the same call gives the same codes.
+ * A gradient that is not finite leaves its block without finite moments.
+ *
+ * `master`, for 16-bit parameters, is the weight itself in fp32; param is then its rounded copy and is only written.
+ * Every array is contiguous and aligned to its element; 16-byte alignment (8 for codes) is what the vector loads want.
+ * Nothing that a step writes may overlap.  Tensors without elements are skipped. */
+typedef struct fbfftconv_adamw fbfftconv_adamw;
+typedef struct fbfftconv_adamw_tensor {
+  void* param;
+  float* master;     /* or null */
+  const void* grad;
+  void* moment1;     /* float*, or uint8_t* codes */
+  void* moment2;
+  float* scale1;     /* null: 32-bit moments */
+  float* scale2;
+  int64_t count;
+  int32_t param_type, grad_type; /* FBFFTCONV_FLOAT32, ... */
+} fbfftconv_adamw_tensor;
+typedef struct fbfftconv_adamw_options {
+  double beta1, beta2, eps, weight_decay;
+  int64_t* steps;    /* device: [0] steps done so far, [1] zero between steps */
+  uint32_t seed;
+  int32_t device;    /* CUDA device ordinal, -1 = current device */
+} fbfftconv_adamw_options;
+/* Checks and copies the list; the arrays stay the caller's and must outlive the handle. */
+int fbfftconv_adamw_create(const fbfftconv_adamw_tensor* tensors, int count, const fbfftconv_adamw_options* options,
+                           fbfftconv_adamw** out);
+int fbfftconv_adamw_destroy(fbfftconv_adamw* h);
+/* Other gradient arrays of the same sizes and types from the next step on. */
+int fbfftconv_adamw_set_gradients(fbfftconv_adamw* h, const void* const* grads, int count);
+/* One step.  scalars, if not null, are two floats on the device, lr and grad_scale, read by the kernel instead of the
+ * arguments: a captured step whose learning rate changes.  Steps of one handle are ordered by the caller (one stream). */
+int fbfftconv_adamw_step(fbfftconv_adamw* h, double lr, float grad_scale, const float* scalars, fbfftconv_stream stream);
+
 /* ---- multi-GPU: one process per GPU ------------------------------------------
  * Replaces the gather / add / broadcast of nn.DataParallel
  * (fbcunn/DataParallel.lua:105-131) by one NCCL all-reduce over NVLink.  Rank 0

@@ -19,7 +19,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libfbfftconv.so")
 SOURCES = ["fft_kernels.cu", "contract_simt.cu", "contract_tc.cu", "contract_stream.cu", "bias.cu", "peer.cu", "tiled.cu", "fft1d_lines.cu",
-           "adamw.cu", "api.cu"]
+           "adamw.cu", "residual_norm.cu", "api.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -95,7 +95,7 @@ def _build_locked(digest: str, verbose: bool) -> None:
             sys.stderr.write(r.stderr)
         return obj
 
-    with ThreadPoolExecutor(max_workers=4) as ex:
+    with ThreadPoolExecutor(max_workers=6) as ex:
         objs = list(ex.map(compile_one, SOURCES))
     tmp = os.path.join(OBJ, "libfbfftconv.so.tmp")
     cmd = [nvcc, "-shared", "-o", tmp, *objs, "-gencode", "arch=compute_100a,code=sm_100a", "-ldl"]

@@ -66,6 +66,20 @@ class AdamwOptions(ctypes.Structure):
     ]
 
 
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+GATE_NONE, GATE_LINEAR, GATE_SIGMOID = 0, 1, 2
+
+
+class NormDesc(ctypes.Structure):
+    """struct fbfftconv_norm_desc."""
+
+    _fields_ = [
+        ("rows", c_int64), ("gate_rows", c_int64), ("u_stride", c_int64), ("r_stride", c_int64), ("gate_stride", c_int64),
+        ("channels", c_int32), ("type", c_int32), ("residual_type", c_int32), ("post", c_int32), ("pre", c_int32),
+        ("gate", c_int32), ("eps", c_float), ("residual_scale", c_float), ("branch_scale", c_float), ("device", c_int32),
+    ]
+
+
 def element_types() -> dict:
     """The element types of the sequence-model operators, by torch type."""
     global _types
@@ -130,6 +144,9 @@ _SIGNATURES = {
     "fbfftconv_adamw_destroy": (c_int, [c_void_p]),
     "fbfftconv_adamw_set_gradients": (c_int, [c_void_p, POINTER(c_void_p), c_int]),
     "fbfftconv_adamw_step": (c_int, [c_void_p, c_double, c_float, c_void_p, c_void_p]),
+    "fbfftconv_residual_norm": (c_int, [c_void_p] * 12),
+    "fbfftconv_residual_norm_workspace_bytes": (c_size_t, [c_void_p]),
+    "fbfftconv_residual_norm_backward": (c_int, [c_void_p] * 17 + [c_float, c_int, c_void_p, c_size_t, c_void_p]),
     "fbfftconv_profile_enable": (c_int, [c_void_p, c_int]),
     "fbfftconv_profile_reset": (c_int, [c_void_p]),
     "fbfftconv_profile_read": (c_int, [c_void_p, c_int, c_int, POINTER(ctypes.c_double), POINTER(c_int)]),

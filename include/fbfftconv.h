@@ -357,6 +357,44 @@ int fbfftconv_adamw_set_gradients(fbfftconv_adamw* h, const void* const* grads, 
  * arguments: a captured step whose learning rate changes.  Steps of one handle are ordered by the caller (one stream). */
 int fbfftconv_adamw_step(fbfftconv_adamw* h, double lr, float grad_scale, const float* scalars, fbfftconv_stream stream);
 
+/* ---- norms before and after a residual block ------------------------------------------------
+ * One call at the border between two blocks of a residual network: the norm after the block that ends, its gate, the
+ * residual sum with its scales, and the norm before the block that begins.
+ *   n = post(u),  r' = residual_scale r + branch_scale act(g) n,  v = pre(r')
+ *   rms(x) = x / sqrt(mean(x^2) + eps) * weight [+ bias],  layer(x) = rms(x - mean(x))
+ * u, r, r', v are (rows, channels); r and r' are the residual stream, of the block's element type or fp32.  v is taken
+ * from the sum before it is rounded to r'.  Either norm may be absent (not both), the gate too.  The gate g has
+ * gate_rows rows, a divisor of rows: consecutive rows / gate_rows rows share one (a gate for each token, sequence, or
+ * for all).  u may be null when neither post-norm nor gate is there: v = pre(r), and r' is r itself, not written.
+ * weights and biases are fp32 (channels); a bias may be null.  channels <= 16384.  Rows of u, r and the gate lie
+ * their stride (elements; 0 = channels) apart, everything else is contiguous. */
+enum { FBFFTCONV_NORM_NONE = 0, FBFFTCONV_NORM_RMS = 1, FBFFTCONV_NORM_LAYER = 2 };
+enum { FBFFTCONV_GATE_NONE = 0, FBFFTCONV_GATE_LINEAR = 1, FBFFTCONV_GATE_SIGMOID = 2 };
+typedef struct fbfftconv_norm_desc {
+  int64_t rows, gate_rows;
+  int64_t u_stride, r_stride, gate_stride;
+  int32_t channels;
+  int32_t type, residual_type;   /* FBFFTCONV_FLOAT32, ... */
+  int32_t post, pre, gate;
+  float eps, residual_scale, branch_scale;
+  int32_t device;                /* CUDA device ordinal, -1 = current device */
+} fbfftconv_norm_desc;
+/* stats: 4 floats a row, 16-byte aligned, for the backward pass; null when there will be none. */
+int fbfftconv_residual_norm(const fbfftconv_norm_desc* desc, const void* u, const void* r, const void* gate,
+                            const float* post_weight, const float* post_bias, const float* pre_weight,
+                            const float* pre_bias, void* r_out, void* v, float* stats, fbfftconv_stream stream);
+/* Bytes of scratch of the backward pass, which the caller lends; calls that may overlap need blocks of their own. */
+size_t fbfftconv_residual_norm_workspace_bytes(const fbfftconv_norm_desc* desc);
+/* Gradients by u, r, gate (of the gate's rows, summed over those that share one), weights and biases from those by r'
+ * and v (grad_r may be null where u is); stats are the forward call's, whose inputs are given again.  The
+ * gradients of weights and biases, each of which may be null, are scaled, and added to where accumulate is set. */
+int fbfftconv_residual_norm_backward(const fbfftconv_norm_desc* desc, const void* u, const void* r, const void* gate,
+                                     const float* stats, const float* post_weight, const float* post_bias,
+                                     const float* pre_weight, const void* grad_r, const void* grad_v, void* grad_u,
+                                     void* grad_r_in, void* grad_gate, float* grad_post_weight, float* grad_post_bias,
+                                     float* grad_pre_weight, float* grad_pre_bias, float scale, int accumulate,
+                                     void* workspace, size_t workspace_bytes, fbfftconv_stream stream);
+
 /* ---- multi-GPU: one process per GPU ------------------------------------------
  * Replaces the gather / add / broadcast of nn.DataParallel
  * (fbcunn/DataParallel.lua:105-131) by one NCCL all-reduce over NVLink.  Rank 0

@@ -80,6 +80,17 @@ class NormDesc(ctypes.Structure):
     ]
 
 
+class RecurrenceDesc(ctypes.Structure):
+    """struct fbfftconv_recurrence_desc."""
+
+    _fields_ = [
+        ("rows", c_int64), ("sequences", c_int64), ("length", c_int64), ("offsets", c_void_p),
+        ("x_stride", c_int64), ("g_stride", c_int64), ("z_stride", c_int64), ("y_stride", c_int64),
+        ("grad_y_stride", c_int64), ("grad_x_stride", c_int64), ("grad_g_stride", c_int64), ("grad_z_stride", c_int64),
+        ("wide_offsets", c_int32), ("channels", c_int32), ("type", c_int32), ("device", c_int32),
+    ]
+
+
 def element_types() -> dict:
     """The element types of the sequence-model operators, by torch type."""
     global _types
@@ -147,6 +158,11 @@ _SIGNATURES = {
     "fbfftconv_residual_norm": (c_int, [c_void_p] * 12),
     "fbfftconv_residual_norm_workspace_bytes": (c_size_t, [c_void_p]),
     "fbfftconv_residual_norm_backward": (c_int, [c_void_p] * 17 + [c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "fbfftconv_recurrence_checkpoint_bytes": (c_size_t, [c_void_p]),
+    "fbfftconv_recurrence_workspace_bytes": (c_size_t, [c_void_p]),
+    "fbfftconv_recurrence": (c_int, [c_void_p] * 10),
+    "fbfftconv_recurrence_backward": (c_int, [c_void_p] * 14 + [c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "fbfftconv_recurrence_step": (c_int, [c_void_p] * 8),
     "fbfftconv_profile_enable": (c_int, [c_void_p, c_int]),
     "fbfftconv_profile_reset": (c_int, [c_void_p]),
     "fbfftconv_profile_read": (c_int, [c_void_p, c_int, c_int, POINTER(ctypes.c_double), POINTER(c_int)]),

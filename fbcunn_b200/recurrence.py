@@ -1,0 +1,196 @@
+"""A gated linear recurrence along sequences, forward, backward and one token at a time.
+
+``GatedLinearRecurrence`` is an nn-style module over fbfftconv_recurrence* (include/fbfftconv.h):
+
+    a_t = sigmoid(g_t + bias),  h_t = a_t h_{t-1} + (1 - a_t) x_t,  y_t = h_t silu(z_t)
+
+updateOutput takes the table [x, g, z] ([x, g] without the output gate: y_t = h_t), padded (batch, length, channels)
+or packed (rows, channels) with offsets; backward the same table and the gradient by y; step one token of every
+sequence with the states in place.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import capi
+from .module import _device_index, _ptr, _stream
+from .residual_norm import _row_stride
+
+
+class GatedLinearRecurrence:
+    """GatedLinearRecurrence(channels): outputGate says whether the table has z, bias whether the gates have a learned
+    one (fp32, zero at first).
+
+    x, g and z are of one type, fp32, bf16 or fp16, and may be parts of one projection's output (rows a common distance
+    apart); gradInput is laid out like that, as parts of one tensor, `gradProjection`.  states are fp32 (sequences,
+    channels): the one after the last row of each sequence is left in `state`, the gradient by the initial one in
+    gradState.  In training() mode, the default, updateOutput leaves in `checkpoints` what backward needs besides its
+    inputs, and backward must follow the updateOutput of the same inputs.  gradBias is overwritten, or added to with
+    accumulate=True."""
+
+    def __init__(self, channels, *, outputGate=True, bias=True, device="cuda", accumulate=False):
+        assert int(channels) > 0, "channels must be positive"
+        self.channels, self.outputGate = int(channels), bool(outputGate)
+        self.device = torch.device(device)
+        self._accumulate = bool(accumulate)
+        self.bias = torch.zeros(self.channels, dtype=torch.float32, device=self.device) if bias else None
+        self.gradBias = torch.zeros_like(self.bias) if bias else None
+        self.train = True
+        self.output = self.state = self.gradInput = self.gradProjection = self.gradState = self.checkpoints = None
+        self._key = None
+        self._step_key = None
+
+    # -- nn.Module surface -------------------------------------------------------
+    def training(self):
+        self.train = True
+
+    def evaluate(self):
+        self.train = False
+
+    def parameters(self):
+        return ([self.bias], [self.gradBias]) if self.bias is not None else ([], [])
+
+    def zeroGradParameters(self):
+        if self.gradBias is not None:
+            self.gradBias.zero_()
+
+    def updateOutput(self, input, state=None, offsets=None):
+        """state: the initial states, or None for zeros; offsets: int32 or int64, sequences + 1 on the device, for packed
+        rows, of which those outside of all sequences stay as they are in `output`."""
+        x, g, z = self._prepare(input, offsets)
+        self._check_state(state, "initial state")
+        if state is not None and state.data_ptr() == self._state.data_ptr():
+            self._state = torch.empty_like(self._state)  # what was returned before is an input now
+        checkpoints = None
+        if self.train:
+            if self._checkpoints is None:
+                n = int(capi.lib().fbfftconv_recurrence_checkpoint_bytes(self._desc_ref))
+                self._checkpoints = torch.empty(max(n // 4, 1), dtype=torch.float32, device=x.device)
+            checkpoints = self._checkpoints
+        capi.check(capi.lib().fbfftconv_recurrence(
+            self._desc_ref, x.data_ptr(), g.data_ptr(), _ptr(z), _ptr(self.bias), _ptr(state), self._output.data_ptr(),
+            self._state.data_ptr(), _ptr(checkpoints), _stream(self._where)))
+        self.output, self.state, self.checkpoints = self._output, self._state, checkpoints
+        return self.output
+
+    def forward(self, input, state=None, offsets=None):
+        return self.updateOutput(input, state, offsets)
+
+    def step(self, input, state):
+        """One token: x, g and z are (sequences, channels), the states are updated in place."""
+        x, g, z = self._table(input)
+        key = (x.shape, x.stride(), g.stride(), None if z is None else z.stride(), x.dtype, x.device)
+        if key != self._step_key:
+            assert x.dim() == 2, "a step takes (sequences, channels)"
+            self._check_table(x, g, z)
+            self._step_desc = self._new_desc(x, g, z, None, x.shape[0], 1)
+            self._step_ref = ctypes.byref(self._step_desc)
+            self._step_output = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            self._step_key = key
+        assert g.shape == x.shape and g.dtype == x.dtype and (z is None or (z.shape == x.shape and z.dtype == x.dtype))
+        assert state.shape == x.shape and state.dtype == torch.float32 and state.is_contiguous() and state.is_cuda
+        capi.check(capi.lib().fbfftconv_recurrence_step(
+            self._step_ref, x.data_ptr(), g.data_ptr(), _ptr(z), _ptr(self.bias), state.data_ptr(),
+            self._step_output.data_ptr(), _stream(x.device)))
+        return self._step_output
+
+    def backward(self, input, gradOutput, scale=None, *, state=None, offsets=None, gradState=None):
+        """The table of gradients; `state` and `offsets` as updateOutput had them, gradState: the gradient by the final
+        states, or None.  With either of the two states, gradState of the module is the one by the initial states."""
+        return self._backward(input, gradOutput, 1.0 if scale is None else float(scale), state, offsets, gradState, True, True)
+
+    def updateGradInput(self, input, gradOutput, *, state=None, offsets=None, gradState=None):
+        return self._backward(input, gradOutput, 1.0, state, offsets, gradState, True, False)
+
+    def accGradParameters(self, input, gradOutput, scale=None, *, state=None, offsets=None, gradState=None):
+        self._backward(input, gradOutput, 1.0 if scale is None else float(scale), state, offsets, gradState, False, True)
+
+    # -- internals -----------------------------------------------------------------
+    def _table(self, input):
+        assert len(input) == (3 if self.outputGate else 2), "the table is [x, g], with the output gate [x, g, z]"
+        return input[0], input[1], input[2] if self.outputGate else None
+
+    def _check_table(self, x, g, z):
+        for t in (x, g, z):
+            if t is None:
+                continue
+            assert isinstance(t, torch.Tensor) and t.is_cuda and t.device == x.device, "CUDA support only!"
+            assert t.dtype in capi.element_types() and t.dtype == x.dtype, "x, g and z have one type: fp32, bf16 or fp16"
+            assert t.shape == x.shape and t.shape[-1] == self.channels, "size mismatch"
+        if self.bias is not None:
+            assert self.bias.device == x.device and self.bias.dtype == torch.float32 and self.bias.is_contiguous()
+            assert self.bias.numel() == self.channels
+
+    def _new_desc(self, x, g, z, offsets, sequences, length):
+        rows = math.prod(x.shape[:-1])
+        return capi.RecurrenceDesc(
+            rows, sequences, length, _ptr(offsets), _row_stride(x), _row_stride(g), _row_stride(z), 0, 0, 0, 0, 0,
+            int(offsets is not None and offsets.dtype == torch.int64), self.channels, capi.element_types()[x.dtype],
+            _device_index(x.device))
+
+    def _prepare(self, input, offsets):
+        """Checks the table; descriptor and outputs are kept for one set of shapes."""
+        x, g, z = self._table(input)
+        key = tuple((t.shape, t.stride(), t.dtype, t.device) if t is not None else None for t in (x, g, z, offsets))
+        if key != self._key:
+            self._check_table(x, g, z)
+            if offsets is None:
+                assert x.dim() == 3, "(batch, length, channels), or packed (rows, channels) with offsets"
+                sequences, length = x.shape[:2]
+            else:
+                assert x.dim() == 2, "packed rows are (rows, channels)"
+                assert offsets.dim() == 1 and offsets.numel() >= 1 and offsets.device == x.device and offsets.is_contiguous()
+                assert offsets.dtype in (torch.int32, torch.int64), "offsets are int32 or int64"
+                sequences, length = offsets.numel() - 1, 0
+            self._desc = self._new_desc(x, g, z, offsets, sequences, length)
+            self._desc_ref = ctypes.byref(self._desc)
+            self._where = x.device
+            self._output = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            self._state = torch.empty((sequences, self.channels), dtype=torch.float32, device=x.device)
+            self._checkpoints = self._grads = None
+            self.checkpoints = None
+            self._key = key
+        if offsets is not None:
+            self._desc.offsets = offsets.data_ptr()
+        return x, g, z
+
+    def _check_state(self, state, what):
+        if state is not None:
+            assert state.shape == self._state.shape and state.dtype == torch.float32 and state.is_contiguous(), \
+                f"the {what} is fp32 (sequences, channels)"
+            assert state.device == self._where, "CUDA support only!"
+
+    def _backward(self, input, gradOutput, scale, state, offsets, gradState, inputs, parameters):
+        kept = self.checkpoints
+        x, g, z = self._prepare(input, offsets)
+        assert kept is not None and self.checkpoints is kept, "updateOutput of the same inputs runs first, in training() mode"
+        self._check_state(state, "initial state")
+        self._check_state(gradState, "gradient by the final state")
+        assert isinstance(gradOutput, torch.Tensor) and gradOutput.is_cuda and gradOutput.device == x.device, "CUDA support only!"
+        assert gradOutput.shape == x.shape and gradOutput.dtype == x.dtype, "gradOutput size mismatch"
+        parts = 3 if self.outputGate else 2
+        if self._grads is None:
+            self._projection = torch.empty(x.shape[:-1] + (parts * self.channels,), dtype=x.dtype, device=x.device)
+            self._grads = list(self._projection.split(self.channels, -1))
+            n = int(capi.lib().fbfftconv_recurrence_workspace_bytes(self._desc_ref))
+            self._workspace = torch.empty(max(n, 16), dtype=torch.uint8, device=x.device)
+            self._grad_state = torch.empty_like(self._state)
+            self._desc.grad_x_stride = self._desc.grad_g_stride = self._desc.grad_z_stride = parts * self.channels
+        self._desc.grad_y_stride = _row_stride(gradOutput)
+        states = inputs and (state is not None or gradState is not None)
+        if states and gradState is not None and gradState.data_ptr() == self._grad_state.data_ptr():
+            self._grad_state = torch.empty_like(self._grad_state)
+        grads = [_ptr(t) if inputs else None for t in self._grads] + [None] * (3 - parts)
+        with_bias = parameters and self.gradBias is not None
+        capi.check(capi.lib().fbfftconv_recurrence_backward(
+            self._desc_ref, x.data_ptr(), g.data_ptr(), _ptr(z), _ptr(self.bias), _ptr(state), kept.data_ptr(),
+            gradOutput.data_ptr(), _ptr(gradState), *grads, self._grad_state.data_ptr() if states else None,
+            self.gradBias.data_ptr() if with_bias else None, scale, int(self._accumulate), self._workspace.data_ptr(),
+            self._workspace.numel(), _stream(self._where)))
+        if inputs:
+            self.gradInput, self.gradProjection = self._grads, self._projection
+            self.gradState = self._grad_state if states else None
+        return self.gradInput

@@ -357,6 +357,45 @@ int fbfftconv_adamw_set_gradients(fbfftconv_adamw* h, const void* const* grads, 
  * arguments: a captured step whose learning rate changes.  Steps of one handle are ordered by the caller (one stream). */
 int fbfftconv_adamw_step(fbfftconv_adamw* h, double lr, float grad_scale, const float* scalars, fbfftconv_stream stream);
 
+/* ---- gated linear recurrence along sequences -------------------------------------------------
+ *   a_t = sigmoid(g_t + bias),  h_t = a_t h_{t-1} + (1 - a_t) x_t,  y_t = h_t silu(z_t)   (y_t = h_t where z is null)
+ * with h_{-1} the sequence's initial state (zero where state0 is null).  x, g, z, y are rows of `channels` neighbours of
+ * one type, their stride (elements; 0 = channels) apart; bias (channels), states (sequences, channels) and checkpoints
+ * are fp32.  The rows are those of `sequences` sequences of `length` rows one behind the other (rows = sequences *
+ * length), or, with offsets (sequences + 1 integers on the device, 32 or with wide_offsets 64 bits wide, not falling),
+ * sequence i has rows [offsets[i], offsets[i + 1]) of `rows`; rows outside of all sequences are neither read nor
+ * written.  Sequences may be empty: their state passes through.  Nothing of a sequence, not even a NaN, reaches the
+ * next.  Results do not depend on the timing of blocks: the same call gives the same bits. */
+typedef struct fbfftconv_recurrence_desc {
+  int64_t rows, sequences, length;
+  const void* offsets;             /* or null */
+  int64_t x_stride, g_stride, z_stride, y_stride;
+  int64_t grad_y_stride, grad_x_stride, grad_g_stride, grad_z_stride;
+  int32_t wide_offsets;
+  int32_t channels;
+  int32_t type;                    /* FBFFTCONV_FLOAT32, ... */
+  int32_t device;                  /* CUDA device ordinal, -1 = current device */
+} fbfftconv_recurrence_desc;
+/* Bytes of the states that the forward pass leaves for the backward pass (one row in 64), and of the scratch that the
+ * backward pass is lent for grad_bias; calls that may overlap need blocks of their own. */
+size_t fbfftconv_recurrence_checkpoint_bytes(const fbfftconv_recurrence_desc* desc);
+size_t fbfftconv_recurrence_workspace_bytes(const fbfftconv_recurrence_desc* desc);
+/* state (the final states) and checkpoints may be null; state must not be state0. */
+int fbfftconv_recurrence(const fbfftconv_recurrence_desc* desc, const void* x, const void* g, const void* z,
+                         const float* bias, const float* state0, void* y, float* state, float* checkpoints,
+                         fbfftconv_stream stream);
+/* Gradients, each of which may be null, from those by y and by the final states (null: zero).  checkpoints are the
+ * forward call's, whose inputs are given again.  grad_bias is scaled, and added to where accumulate is set; workspace
+ * may be null without it. */
+int fbfftconv_recurrence_backward(const fbfftconv_recurrence_desc* desc, const void* x, const void* g, const void* z,
+                                  const float* bias, const float* state0, const float* checkpoints, const void* grad_y,
+                                  const float* grad_state, void* grad_x, void* grad_g, void* grad_z, float* grad_state0,
+                                  float* grad_bias, float scale, int accumulate, void* workspace, size_t workspace_bytes,
+                                  fbfftconv_stream stream);
+/* One row of every sequence (length 1, no offsets), the states updated in place: what serving does for each token. */
+int fbfftconv_recurrence_step(const fbfftconv_recurrence_desc* desc, const void* x, const void* g, const void* z,
+                              const float* bias, float* state, void* y, fbfftconv_stream stream);
+
 /* ---- norms before and after a residual block ------------------------------------------------
  * One call at the border between two blocks of a residual network: the norm after the block that ends, its gate, the
  * residual sum with its scales, and the norm before the block that begins.

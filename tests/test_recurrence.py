@@ -1,0 +1,95 @@
+"""The recurrence's entry points refuse bad arguments before they touch a device, and its search over packed sequences
+stays in bounds and ends for whatever the offsets hold (a host's copy of the kernel's index arithmetic)."""
+import ctypes
+import random
+
+import pytest
+
+from fbcunn_b200 import build as fb_build
+from fbcunn_b200 import capi
+
+
+@pytest.fixture(scope="module")
+def lib():
+    fb_build.build()
+    return capi.lib()
+
+
+def _desc(**kw):
+    base = dict(rows=12, sequences=3, length=4, channels=64, type=capi.BFLOAT16, device=0)
+    return capi.RecurrenceDesc(**{**base, **kw})
+
+
+BAD = [dict(channels=0), dict(channels=-4), dict(channels=(1 << 22) + 1), dict(rows=-1), dict(sequences=-1), dict(length=-1),
+       dict(type=5), dict(rows=13), dict(length=5), dict(length=0), dict(sequences=1 << 32, length=1 << 32, rows=0),
+       dict(offsets=4098), dict(offsets=4100, wide_offsets=1), dict(rows=1 << 41, offsets=4096)]
+
+
+@pytest.mark.parametrize("bad", range(len(BAD)))
+def test_bad_descriptors(lib, bad):
+    d = ctypes.byref(_desc(**BAD[bad]))
+    refused = (capi.ERR_INVALID_ARGUMENT, capi.ERR_UNSUPPORTED_SIZE)
+    assert lib.fbfftconv_recurrence(d, *[4096] * 8, None) in refused
+    assert lib.fbfftconv_recurrence_backward(d, *[4096] * 13, 1.0, 0, 4096, 1 << 20, None) in refused
+    assert lib.fbfftconv_recurrence_step(d, *[4096] * 6, None) in refused
+    assert lib.fbfftconv_recurrence_checkpoint_bytes(d) == 0 and lib.fbfftconv_recurrence_workspace_bytes(d) == 0
+
+
+def test_bad_pointers(lib):
+    d = ctypes.byref(_desc())
+    good = [4096, 8192, 12288, 16384, 20480, 24576, 28672, 32768]
+    for i, value in [(0, None), (1, None), (5, None), (0, 4097), (2, 4097), (3, 4098), (4, 4098), (6, 20480), (7, 4098)]:
+        args = list(good)
+        args[i] = value
+        assert lib.fbfftconv_recurrence(d, *args, None) == capi.ERR_INVALID_ARGUMENT
+    overlap = ctypes.byref(_desc(x_stride=32))
+    assert lib.fbfftconv_recurrence(overlap, *good, None) == capi.ERR_INVALID_ARGUMENT and "overlap" in capi.last_error()
+    args = [4096 * (i + 1) for i in range(13)]
+    assert lib.fbfftconv_recurrence_backward(d, *args, float("inf"), 0, 4096, 1 << 20, None) == capi.ERR_INVALID_ARGUMENT
+    no_z = list(args)
+    no_z[2] = None
+    assert lib.fbfftconv_recurrence_backward(d, *no_z, 1.0, 0, 4096, 1 << 20, None) == capi.ERR_INVALID_ARGUMENT
+    shared = list(args)
+    shared[11] = shared[7]
+    assert lib.fbfftconv_recurrence_backward(d, *shared, 1.0, 0, 4096, 1 << 20, None) == capi.ERR_INVALID_ARGUMENT
+    assert lib.fbfftconv_recurrence_step(d, *good[:6], None) == capi.ERR_INVALID_ARGUMENT  # length 4
+
+
+def test_search_over_any_offsets():
+    rng = random.Random(1)
+    for trial in range(3000):
+        rows, n = rng.randint(1, 60), rng.randint(1, 9)
+        offsets = [rng.choice([rng.randint(0, rows), rng.randint(-100, 100), 1 << 40]) for _ in range(n + 1)]
+        if trial % 3 == 0:
+            offsets = sorted(rng.randint(0, rows) for _ in range(n + 1))
+        at = lambda i: min(max(offsets[i], 0), rows)
+        def sequence_of(row):
+            lo, hi = 0, n
+            while hi - lo > 1:
+                mid = (lo + hi) // 2
+                lo, hi = (mid, hi) if at(mid) <= row else (lo, mid)
+            assert 0 <= lo < n
+            return at(lo), at(lo + 1)
+        begin, end = at(0), at(n)
+        for row in range(begin, end, 16):
+            count, first, last, turns = min(16, end - row), 0, 0, 0
+            lo, hi = sequence_of(row)
+            first = int(row == lo)
+            while hi > row and hi - row <= count:
+                turns += 1
+                assert turns <= 17, "no end"
+                k = hi - row
+                last |= 1 << (k - 1)
+                if k == count:
+                    break
+                first |= 1 << k
+                lo, more = sequence_of(hi)
+                if more <= hi:
+                    break
+                hi = more
+            assert first < 1 << count and last < 1 << count
+            if trial % 3 == 0:  # sorted: exactly the rows that begin and end a sequence
+                starts = {offsets[i] for i in range(n) if offsets[i] < offsets[i + 1]}
+                ends = {offsets[i + 1] - 1 for i in range(n) if offsets[i] < offsets[i + 1]}
+                assert [first >> i & 1 for i in range(count)] == [int(row + i in starts) for i in range(count)]
+                assert [last >> i & 1 for i in range(count)] == [int(row + i in ends) for i in range(count)]

@@ -16,6 +16,7 @@
 #include <cooperative_groups.h>
 #include <math.h>
 
+#include <mutex>
 #include <type_traits>
 
 #include "operators.cuh"
@@ -28,7 +29,7 @@ namespace {
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kForwardRows = 16, kBackwardRows = 8;  // of a warp, in a round
 constexpr int kCheckpoint = 64;                      // rows between the states that forward leaves for backward
-constexpr int kMostCluster = 8;
+constexpr int kMostCluster = 16;
 static_assert(kCheckpoint % kForwardRows == 0 && kWarps * kBackwardRows == kCheckpoint && (kWarps * kForwardRows) % kCheckpoint == 0);
 
 struct RecArgs {
@@ -80,158 +81,241 @@ __device__ __forceinline__ Sequence sequence_of(const RecArgs& a, long long row)
   return {lo, offset_at(a, lo), offset_at(a, lo + 1)};
 }
 
-// Which of n rows from `row` on begin a sequence, and which end one.
-__device__ __forceinline__ void borders(const RecArgs& a, long long row, int n, uint32_t& first, uint32_t& last) {
-  first = last = 0;
-  if (n <= 0) return;
-  Sequence s = sequence_of(a, row);
-  if (row == s.begin) first = 1;
-  while (s.end > row && s.end - row <= n) {
-    const int k = (int)(s.end - row);
-    last |= 1u << (k - 1);
+// The sequence that a row belongs to, for the few rows that begin or end one: kept out of the loops' code.
+__device__ __noinline__ long long index_of(const RecArgs& a, long long row) { return sequence_of(a, row).index; }
+
+// Which of a warp's rows begin a sequence, and which end one.  `in`, the sequence that its rows were in last, is looked
+// up anew only where they have left it; most rounds lie within one sequence.
+struct Borders {
+  uint32_t first, last;
+};
+__device__ __forceinline__ Borders borders(const RecArgs& a, long long row, int n, Sequence& in) {
+  Borders b{0, 0};
+  if (n <= 0) return b;
+  if (row < in.begin || row >= in.end) in = sequence_of(a, row);
+  if (row > in.begin && in.end - row > n) return b;
+  if (row == in.begin) b.first = 1;
+  while (in.end > row && in.end - row <= n) {
+    const int k = (int)(in.end - row);
+    b.last |= 1u << (k - 1);
     if (k == n) break;
-    first |= 1u << k;
-    const Sequence next = sequence_of(a, s.end);
-    if (next.end <= s.end) break;  // offsets that do not rise
-    s = next;
+    b.first |= 1u << k;
+    const Sequence next = sequence_of(a, in.end);
+    if (next.end <= in.end) break;  // offsets that do not rise
+    in = next;
   }
+  return b;
+}
+
+// A lane's channels: one value, or two whose sums and products are single instructions (the issue slots are what runs
+// out first here).
+template <int V> struct Vec;
+template <> struct Vec<1> {
+  float x;
+  __device__ __forceinline__ float get(int) const { return x; }
+  __device__ __forceinline__ void set(int, float v) { x = v; }
+};
+template <> struct Vec<2> {
+  float x, y;
+  __device__ __forceinline__ float get(int i) const { return i ? y : x; }
+  __device__ __forceinline__ void set(int i, float v) { (i ? y : x) = v; }
+  __device__ __forceinline__ unsigned long long bits() const {
+    unsigned long long b;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "f"(x), "f"(y));
+    return b;
+  }
+  static __device__ __forceinline__ Vec from(unsigned long long b) {
+    Vec v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(b));
+    return v;
+  }
+};
+template <int V> __device__ __forceinline__ Vec<V> all_of(float v) {
+  Vec<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.set(i, v);
+  return r;
+}
+__device__ __forceinline__ Vec<1> fma(Vec<1> a, Vec<1> b, Vec<1> c) { return {fmaf(a.x, b.x, c.x)}; }
+__device__ __forceinline__ Vec<1> operator*(Vec<1> a, Vec<1> b) { return {a.x * b.x}; }
+__device__ __forceinline__ Vec<1> operator+(Vec<1> a, Vec<1> b) { return {a.x + b.x}; }
+__device__ __forceinline__ Vec<2> fma(Vec<2> a, Vec<2> b, Vec<2> c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a.bits()), "l"(b.bits()), "l"(c.bits()));
+  return Vec<2>::from(d);
+}
+__device__ __forceinline__ Vec<2> operator*(Vec<2> a, Vec<2> b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.bits()), "l"(b.bits()));
+  return Vec<2>::from(d);
+}
+__device__ __forceinline__ Vec<2> operator+(Vec<2> a, Vec<2> b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.bits()), "l"(b.bits()));
+  return Vec<2>::from(d);
 }
 
 // h -> A h + H; A < 0 stands for rows that begin a sequence among them: nothing of h comes through, not even a NaN.
-struct Stretch {
-  float A, H;
+template <int V> struct Stretch {
+  Vec<V> A, H;
 };
-__device__ __forceinline__ float apply(const Stretch& s, float h) { return s.A < 0.f ? s.H : fmaf(s.A, h, s.H); }
-__device__ __forceinline__ Stretch join(const Stretch& s, const Stretch& next) {
-  return {next.A < 0.f || s.A < 0.f ? -1.f : s.A * next.A, apply(next, s.H)};
+template <int V> __device__ __forceinline__ Vec<V> apply(const Stretch<V>& s, Vec<V> h) {
+  Vec<V> r = fma(s.A, h, s.H);
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (s.A.get(v) < 0.f) r.set(v, s.H.get(v));
+  return r;
 }
+template <int V> __device__ __forceinline__ Stretch<V> join(const Stretch<V>& s, const Stretch<V>& next) {
+  Stretch<V> r{s.A * next.A, apply(next, s.H)};
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (s.A.get(v) < 0.f || next.A.get(v) < 0.f) r.A.set(v, -1.f);
+  return r;
+}
+template <int V> __device__ __forceinline__ Stretch<V> nothing() { return {all_of<V>(1.f), all_of<V>(0.f)}; }
 
 __device__ __forceinline__ float reciprocal(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-
-// a = sigmoid(g) and b = 1 - a, both to the last places: the larger is formed from the smaller.
-__device__ __forceinline__ void gate_of(float g, float& a, float& b) {
-  const float e = __expf(-fabsf(g));
-  const float small = e * reciprocal(1.f + e), big = 1.f - small;
-  a = g < 0.f ? small : big;
-  b = g < 0.f ? big : small;
+__device__ __forceinline__ float exp2_fast(float x) {  // results below the normal numbers are zero
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return reciprocal(1.f + __expf(-x)); }
+constexpr float kLog2e = 1.4426950408889634f;
+
+// a = sigmoid(g) and b = 1 - a, both to the last places: the larger is formed from the smaller.
+template <int V> __device__ __forceinline__ void gate_of(Vec<V> g, Vec<V>& a, Vec<V>& b) {
+  Vec<V> e, r;
+#pragma unroll
+  for (int v = 0; v < V; ++v) e.set(v, exp2_fast(-kLog2e * fabsf(g.get(v))));
+  const Vec<V> d = e + all_of<V>(1.f);
+#pragma unroll
+  for (int v = 0; v < V; ++v) r.set(v, reciprocal(d.get(v)));
+  const Vec<V> small = e * r, big = fma(small, all_of<V>(-1.f), all_of<V>(1.f));
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    a.set(v, g.get(v) < 0.f ? small.get(v) : big.get(v));
+    b.set(v, g.get(v) < 0.f ? big.get(v) : small.get(v));
+  }
+}
+
+template <int V> __device__ __forceinline__ Vec<V> sigmoid(Vec<V> x) {
+  const Vec<V> t = x * all_of<V>(-kLog2e);
+  Vec<V> e, r;
+#pragma unroll
+  for (int v = 0; v < V; ++v) e.set(v, exp2_fast(t.get(v)));
+  e = e + all_of<V>(1.f);
+#pragma unroll
+  for (int v = 0; v < V; ++v) r.set(v, reciprocal(e.get(v)));
+  return r;
+}
+
+template <int V> __device__ __forceinline__ Vec<V> load_floats(const float* p) {
+  Vec<V> r;
+#pragma unroll
+  for (int v = 0; v < V; ++v) r.set(v, p[v]);
+  return r;
+}
+template <int V> __device__ __forceinline__ void store_floats(float* p, Vec<V> x) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) p[v] = x.get(v);
+}
 
 // A lane's channels of a row: one 32-bit word, or a single 16-bit value where pairs are not aligned.
-template <typename T, int V> __device__ __forceinline__ void unpack(uint32_t w, float (&x)[V]) {
+template <typename T, int V> __device__ __forceinline__ Vec<V> unpack(uint32_t w) {
   if constexpr (std::is_same_v<T, float>) {
-    x[0] = __uint_as_float(w);
+    return Vec<1>{__uint_as_float(w)};
   } else if constexpr (V == 2) {
     const float2 f = unpack2<T>(w);
-    x[0] = f.x, x[1] = f.y;
+    return Vec<2>{f.x, f.y};
   } else {
-    x[0] = unpack2<T>(w).x;
+    return Vec<1>{unpack2<T>(w).x};
   }
 }
 template <typename T, int V> __device__ __forceinline__ uint32_t load_word(const T* p) {
   if constexpr (sizeof(T) * V == 4) return __ldg(reinterpret_cast<const uint32_t*>(p));
   else return __ldg(reinterpret_cast<const uint16_t*>(p));
 }
-template <typename T, int V> __device__ __forceinline__ void store_word(T* p, const float (&x)[V]) {
-  if constexpr (std::is_same_v<T, float>) *p = x[0];
-  else if constexpr (V == 2) *reinterpret_cast<uint32_t*>(p) = pack2<T>(x[0], x[1]);
-  else *p = from_float<T>(x[0]);
+template <typename T, int V> __device__ __forceinline__ void store_word(T* p, Vec<V> x) {
+  if constexpr (std::is_same_v<T, float>) *p = x.x;
+  else if constexpr (V == 2) *reinterpret_cast<uint32_t*>(p) = pack2<T>(x.x, x.y);
+  else *p = from_float<T>(x.x);
 }
 
-// The words of a thread's next rows: in shared memory, on their way there while this round is computed.  Single 16-bit
-// values, which cp.async does not copy, are loaded where they are read.
-template <typename T, int V, int kRows, int kStreams>
+// The words of a thread's next rows: in shared memory, on their way there while this round is computed.  A slot holds
+// one tensor's rows; it is filled anew as soon as the round has read it, one group of copies after the scan and one
+// after the outputs, so that the oldest group but one is always the one that is waited for.  Single 16-bit values,
+// which cp.async does not copy, are loaded where they are read.
+template <typename T, int V, int kRows>
 struct Words {
   static constexpr bool kAsync = sizeof(T) * V == 4;
-  static constexpr int kStage = kStreams * kRows * kThreads * 4;
+  static constexpr int kSlot = kRows * kThreads * 4;
   char* base;  // this thread's
-  const T* at[kStreams];      // the thread's channels of row 0
-  long long stride[kStreams];
 
-  __device__ __forceinline__ void fetch(int stage, long long row, int n, bool on) const {
+  __device__ __forceinline__ void fetch(int slot, const T* p, long long stride, int n) const {
     if constexpr (kAsync) {
-      if (on) {
+      const uint32_t to = (uint32_t)__cvta_generic_to_shared(base + slot * kSlot);
+      const auto copy = [&](auto all) {
 #pragma unroll
-        for (int s = 0; s < kStreams; ++s) {
-          const T* p = at[s] + row * stride[s];
-          const uint32_t to = (uint32_t)__cvta_generic_to_shared(base + stage * kStage + s * kRows * kThreads * 4);
-#pragma unroll
-          for (int i = 0; i < kRows; ++i)
-            if (i < n)
-              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + i * kThreads * 4), "l"(p + i * stride[s]) : "memory");
-        }
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+        for (int i = 0; i < kRows; ++i)
+          if (all || i < n)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + i * kThreads * 4), "l"(p + i * stride) : "memory");
+      };
+      if (n == kRows) copy(std::true_type{});
+      else copy(std::false_type{});
     }
+  }
+  __device__ __forceinline__ void commit() const {
+    if constexpr (kAsync) asm volatile("cp.async.commit_group;" ::: "memory");
   }
   __device__ __forceinline__ void wait() const {
     if constexpr (kAsync) asm volatile("cp.async.wait_group 1;" ::: "memory");
   }
-  // i below the rows that there are
-  __device__ __forceinline__ void read(int stage, int s, long long row, int i, float (&x)[V]) const {
-    if constexpr (kAsync) unpack<T, V>(*reinterpret_cast<const uint32_t*>(base + stage * kStage + (s * kRows + i) * kThreads * 4), x);
-    else unpack<T, V>(load_word<T, V>(at[s] + (row + i) * stride[s]), x);
+  // row i of the slot, which is that of `p`
+  __device__ __forceinline__ Vec<V> read(int slot, const T* p, long long stride, int i) const {
+    if constexpr (kAsync) return unpack<T, V>(*reinterpret_cast<const uint32_t*>(base + slot * kSlot + i * kThreads * 4));
+    else return unpack<T, V>(load_word<T, V>(p + i * stride));
   }
 };
 
 // Joins what the warps and blocks before one have: a block's warps through `part`, a cluster's blocks through `whole`.
-// "Before" is in the direction of the scan; `order` counts in it.  Two halves are used in turn.
+// "Before" is in the direction of the scan; `order` counts in it.  Two buffers are used in turn where nothing but the
+// next round's barrier separates a round's reads from the next one's writes.
 template <int V>
 struct Exchange {
-  Stretch part[2][kWarps][32][V];
-  Stretch whole[2][kMostCluster][32][V];
+  Stretch<V> part[kWarps][32];
+  Stretch<V> whole[2][kMostCluster][32];
 };
 
 // `mine`: this warp's stretch; returns the value that enters it and moves `carry` behind the whole round.
 template <int V>
-__device__ __forceinline__ void exchange(Exchange<V>& x, int half, int order, int rank, int blocks, const Stretch (&mine)[V],
-                                         float (&carry)[V], float (&enter)[V]) {
+__device__ __forceinline__ Vec<V> exchange(Exchange<V>& x, int half, int order, int rank, int blocks, const Stretch<V>& mine,
+                                           Vec<V>& carry) {
   const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int v = 0; v < V; ++v) x.part[half][order][lane][v] = mine[v];
+  Stretch<V>(*const part)[32] = blocks == 1 && half ? x.whole[0] : x.part;
+  part[order][lane] = mine;
   __syncthreads();
-  Stretch before[V], all[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) all[v] = before[v] = Stretch{1.f, 0.f};
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if (w == order) before[v] = all[v];
-      all[v] = join(all[v], x.part[half][w][lane][v]);
-    }
-  }
+  Stretch<V> before = nothing<V>();
+  for (int w = 0; w < order; ++w) before = join(before, part[w][lane]);
+  Stretch<V> all = join(before, mine);
+  for (int w = order + 1; w < kWarps; ++w) all = join(all, part[w][lane]);
   if (blocks == 1) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      enter[v] = apply(before[v], carry[v]);
-      carry[v] = apply(all[v], carry[v]);
-    }
-    return;
+    const Vec<V> enter = apply(before, carry);
+    carry = apply(all, carry);
+    return enter;
   }
   cg::cluster_group cluster = cg::this_cluster();
-  if (order < blocks) {
-    Exchange<V>* const other = cluster.map_shared_rank(&x, order);
-#pragma unroll
-    for (int v = 0; v < V; ++v) other->whole[half][rank][lane][v] = all[v];
-  }
+  for (int k = order; k < blocks; k += kWarps) cluster.map_shared_rank(&x, k)->whole[half][rank][lane] = all;
   cluster.sync();
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    float h = carry[v];
-    enter[v] = h;
-    for (int k = 0; k < blocks; ++k) {
-      if (k == rank) enter[v] = h;
-      h = apply(x.whole[half][k][lane][v], h);
-    }
-    enter[v] = apply(before[v], enter[v]);
-    carry[v] = h;
-  }
+  for (int k = 0; k < rank; ++k) carry = apply(x.whole[half][k][lane], carry);
+  const Vec<V> enter = apply(before, carry);
+  for (int k = rank; k < blocks; ++k) carry = apply(x.whole[half][k][lane], carry);
+  return enter;
 }
 
 // The rows of this block's segment: [begin, end).
@@ -259,8 +343,8 @@ __device__ __forceinline__ void pass_empty(const RecArgs& a, const float* from, 
 }
 
 template <typename T, int V, bool kGate>
-__global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const RecArgs a) {
-  constexpr int L = kForwardRows, kTile = kWarps * L, kStreams = kGate ? 3 : 2;
+__global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const __grid_constant__ RecArgs a) {
+  constexpr int L = kForwardRows, kTile = kWarps * L;
   extern __shared__ __align__(16) char staged[];
   __shared__ Exchange<V> shared;
   grid_dependency_wait();
@@ -273,96 +357,95 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const R
   segment_rows(a, begin, end);
   if (rank == 0) pass_empty<V>(a, a.state0, a.state, c, on);
   const long long tiles = (end - begin + kTile - 1) / kTile, rounds = (tiles + blocks - 1) / blocks;
-  Words<T, V, L, kStreams> words;
-  words.base = staged + 4 * threadIdx.x;
-  words.at[0] = static_cast<const T*>(a.x) + c, words.stride[0] = a.x_stride;
-  words.at[1] = static_cast<const T*>(a.g) + c, words.stride[1] = a.g_stride;
-  if (kGate) words.at[kStreams - 1] = static_cast<const T*>(a.z) + c, words.stride[kStreams - 1] = a.z_stride;
-  float bias[V], carry[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) bias[v] = a.bias ? a.bias[c + v] : 0.f, carry[v] = 0.f;
+  const Words<T, V, L> words{staged + 4 * threadIdx.x};
+  enum { kX, kG, kZ };  // slots
+  const T* const x0 = static_cast<const T*>(a.x) + c;
+  const T* const g0 = static_cast<const T*>(a.g) + c;
+  const T* const z0 = static_cast<const T*>(a.z) + c;
+  const Vec<V> bias = a.bias ? load_floats<V>(a.bias + c) : all_of<V>(0.f);
+  Vec<V> carry = all_of<V>(0.f);
   const auto row_of = [&](long long round) { return begin + ((round * blocks + rank) * kWarps + warp) * L; };
   const auto rows_at = [&](long long row) { return (int)max(0ll, min((long long)L, end - row)); };
-  for (int k = 0; k < 2; ++k) words.fetch(k, row_of(k), rows_at(row_of(k)), on);
+  const auto fetch_inputs = [&](long long round) {
+    const long long row = row_of(round);
+    const int n = on ? rows_at(row) : 0;
+    words.fetch(kX, x0 + row * a.x_stride, a.x_stride, n);
+    words.fetch(kG, g0 + row * a.g_stride, a.g_stride, n);
+    words.commit();
+  };
+  const auto fetch_outputs = [&](long long round) {
+    const long long row = row_of(round);
+    if (kGate) words.fetch(kZ, z0 + row * a.z_stride, a.z_stride, on ? rows_at(row) : 0);
+    words.commit();
+  };
+  fetch_inputs(0);
+  fetch_outputs(0);
+  Sequence in{0, 0, 0};
   for (long long round = 0; round < rounds; ++round) {
-    const int stage = (int)(round & 1);
     const long long row = row_of(round);
     const int n = rows_at(row);
+    const T* const xs = x0 + row * a.x_stride;
+    const T* const gs = g0 + row * a.g_stride;
+    const T* const zs = z0 + row * a.z_stride;
     words.wait();
-    uint32_t first, last;
-    borders(a, row, n, first, last);
-    float A[L][V], B[L][V];
-    Stretch mine[V];
+    const Borders at = borders(a, row, n, in);
+    const bool within = n == L && at.first == 0 && at.last == 0;  // all rows there, none at a sequence's border
+    Vec<V> A[L], B[L];
+    Stretch<V> mine = nothing<V>();
+    const auto scan = [&](auto plain) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) mine[v] = Stretch{1.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      if (i < n) {
-        float x[V], g[V];
-        words.read(stage, 0, row, i, x);
-        words.read(stage, 1, row, i, g);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          gate_of(g[v] + bias[v], A[i][v], B[i][v]);
-          B[i][v] *= x[v];
-        }
-        if (first >> i & 1) {  // the row takes the initial state, whatever comes before it
-          const float* const h0 = a.state0 ? a.state0 + sequence_of(a, row + i).index * a.channels + c : nullptr;
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            B[i][v] = h0 ? fmaf(A[i][v], h0[v], B[i][v]) : B[i][v];
-            mine[v] = Stretch{-1.f, B[i][v]};
+      for (int i = 0; i < L; ++i) {
+        if (plain || i < n) {
+          gate_of(words.read(kG, gs, a.g_stride, i) + bias, A[i], B[i]);
+          B[i] = B[i] * words.read(kX, xs, a.x_stride, i);
+          if (!plain && (at.first >> i & 1)) {  // the row takes the initial state, whatever comes before it
+            if (a.state0) B[i] = fma(A[i], load_floats<V>(a.state0 + index_of(a, row + i) * a.channels + c), B[i]);
+            mine = Stretch<V>{all_of<V>(-1.f), B[i]};
+          } else {
+            const bool cut = !plain && mine.A.x < 0.f;
+            mine = Stretch<V>{cut ? mine.A : mine.A * A[i], fma(A[i], mine.H, B[i])};
           }
         } else {
-#pragma unroll
-          for (int v = 0; v < V; ++v) mine[v] = Stretch{mine[v].A < 0.f ? -1.f : mine[v].A * A[i][v], fmaf(A[i][v], mine[v].H, B[i][v])};
+          A[i] = all_of<V>(1.f), B[i] = all_of<V>(0.f);
         }
-      } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) A[i][v] = 1.f, B[i][v] = 0.f;
       }
-    }
-    float h[V];
-    exchange(shared, stage, warp, rank, blocks, mine, carry, h);
-    if (a.checkpoints && n > 0 && on && (row - begin) % kCheckpoint == 0) {
-      float* const to = a.checkpoints + (blockIdx.y * a.checkpoints_per_segment + (row - begin) / kCheckpoint) * a.channels + c;
-#pragma unroll
-      for (int v = 0; v < V; ++v) to[v] = h[v];
-    }
+    };
+    if (within) scan(std::true_type{});
+    else scan(std::false_type{});
+    fetch_inputs(round + 1);
+    Vec<V> h = exchange(shared, (int)(round & 1), warp, rank, blocks, mine, carry);
+    words.wait();
+    if (a.checkpoints && n > 0 && on && (row - begin) % kCheckpoint == 0)
+      store_floats(a.checkpoints + (blockIdx.y * a.checkpoints_per_segment + (row - begin) / kCheckpoint) * a.channels + c, h);
     T* y = static_cast<T*>(a.y) + row * a.y_stride + c;
+    const auto emit = [&](auto plain) {
 #pragma unroll
-    for (int i = 0; i < L; ++i) {
-      if (i >= n) continue;
-      const bool start = first >> i & 1;
-#pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = start ? B[i][v] : fmaf(A[i][v], h[v], B[i][v]);
-      float out[V];
-      if (kGate) {
-        float z[V];
-        words.read(stage, kStreams - 1, row, i, z);
-#pragma unroll
-        for (int v = 0; v < V; ++v) out[v] = h[v] * (z[v] * sigmoid(z[v]));
-      } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) out[v] = h[v];
+      for (int i = 0; i < L; ++i) {
+        if (!plain && i >= n) continue;
+        const bool start = !plain && (at.first >> i & 1);
+        h = start ? B[i] : fma(A[i], h, B[i]);
+        Vec<V> out = h;
+        if (kGate) {
+          const Vec<V> z = words.read(kZ, zs, a.z_stride, i);
+          out = (h * z) * sigmoid(z);
+        }
+        if (on) store_word<T, V>(y + i * a.y_stride, out);
+        if (!plain && (at.last >> i & 1) && a.state && on)
+          store_floats(a.state + index_of(a, row + i) * a.channels + c, h);
       }
-      if (on) store_word<T, V>(y + i * a.y_stride, out);
-      if ((last >> i & 1) && a.state && on) {
-        float* const to = a.state + sequence_of(a, row + i).index * a.channels + c;
-#pragma unroll
-        for (int v = 0; v < V; ++v) to[v] = h[v];
-      }
-    }
-    words.fetch(stage, row_of(round + 2), rows_at(row_of(round + 2)), on);
+    };
+    if (within) emit(std::true_type{});
+    else emit(std::false_type{});
+    fetch_outputs(round + 1);
   }
 }
 
 template <typename T, int V, bool kGate>
-__global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const RecArgs a) {
-  constexpr int L = kBackwardRows, kTile = kWarps * L, kStreams = kGate ? 4 : 3;
+__global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const __grid_constant__ RecArgs a) {
+  constexpr int L = kBackwardRows, kTile = kWarps * L;
   extern __shared__ __align__(16) char staged[];
   __shared__ Exchange<V> shared;
-  __shared__ Stretch states[2][kWarps][32][V];
+  __shared__ Stretch<V> states[2][kWarps][32];
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int blocks = a.cluster, rank = blockIdx.x % blocks;
@@ -373,159 +456,144 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
   segment_rows(a, begin, end);
   if (rank == 0) pass_empty<V>(a, a.dstate, a.dstate0, c, on);
   const long long tiles = (end - begin + kTile - 1) / kTile, rounds = (tiles + blocks - 1) / blocks;
-  Words<T, V, L, kStreams> words;
-  words.base = staged + 4 * threadIdx.x;
-  words.at[0] = static_cast<const T*>(a.x) + c, words.stride[0] = a.x_stride;
-  words.at[1] = static_cast<const T*>(a.g) + c, words.stride[1] = a.g_stride;
-  words.at[2] = static_cast<const T*>(a.dy) + c, words.stride[2] = a.dy_stride;
-  if (kGate) words.at[kStreams - 1] = static_cast<const T*>(a.z) + c, words.stride[kStreams - 1] = a.z_stride;
-  float bias[V], carry[V], dbias[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) bias[v] = a.bias ? a.bias[c + v] : 0.f, carry[v] = dbias[v] = 0.f;
+  const Words<T, V, L> words{staged + 4 * threadIdx.x};
+  enum { kX, kG = 2, kDy, kZ };  // slots: x has two, it is read to the end of its round
+  const T* const x0 = static_cast<const T*>(a.x) + c;
+  const T* const g0 = static_cast<const T*>(a.g) + c;
+  const T* const dy0 = static_cast<const T*>(a.dy) + c;
+  const T* const z0 = static_cast<const T*>(a.z) + c;
+  const Vec<V> bias = a.bias ? load_floats<V>(a.bias + c) : all_of<V>(0.f);
+  Vec<V> carry = all_of<V>(0.f), dbias = all_of<V>(0.f);
   // the last rows come first
   const auto tile_of = [&](long long round) { return tiles - 1 - (round * blocks + rank); };
   const auto row_of = [&](long long round) { return begin + (tile_of(round) * kWarps + warp) * L; };
   const auto rows_at = [&](long long round) { return tile_of(round) < 0 ? 0 : (int)max(0ll, min((long long)L, end - row_of(round))); };
-  for (int k = 0; k < 2; ++k) words.fetch(k, row_of(k), rows_at(k), on);
+  const auto fetch_inputs = [&](long long round) {
+    const long long row = row_of(round);
+    const int n = on ? rows_at(round) : 0;
+    words.fetch(kX + (int)(round & 1), x0 + row * a.x_stride, a.x_stride, n);
+    words.fetch(kG, g0 + row * a.g_stride, a.g_stride, n);
+    words.commit();
+  };
+  const auto fetch_outputs = [&](long long round) {
+    const long long row = row_of(round);
+    const int n = on ? rows_at(round) : 0;
+    words.fetch(kDy, dy0 + row * a.dy_stride, a.dy_stride, n);
+    if (kGate) words.fetch(kZ, z0 + row * a.z_stride, a.z_stride, n);
+    words.commit();
+  };
+  fetch_inputs(0);
+  fetch_outputs(0);
+  Sequence in{0, 0, 0};
   for (long long round = 0; round < rounds; ++round) {
     const int stage = (int)(round & 1);
     const long long row = row_of(round), tile = tile_of(round);
     const int n = rows_at(round);
-    float entered[V];  // the state before the tile
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      entered[v] = tile < 0 ? 0.f : a.checkpoints[(blockIdx.y * a.checkpoints_per_segment + tile) * a.channels + c + v];
+    const T* const xs = x0 + row * a.x_stride;
+    const T* const gs = g0 + row * a.g_stride;
+    const T* const dys = dy0 + row * a.dy_stride;
+    const T* const zs = z0 + row * a.z_stride;
+    // the state before the tile
+    Vec<V> h = tile < 0 ? all_of<V>(0.f)
+                        : load_floats<V>(a.checkpoints + (blockIdx.y * a.checkpoints_per_segment + tile) * a.channels + c);
     words.wait();
-    uint32_t first, last;
-    borders(a, row, n, first, last);
+    const Borders at = borders(a, row, n, in);
+    const bool within = n == L && at.first == 0 && at.last == 0;  // all rows there, none at a sequence's border
     // the states of the warp's rows: its stretch, those of the warps before it, and from row to row
-    float A[L][V], B[L][V], P[L][V], E[L][V];  // gates, states before each row, what enters each row from its output
-    Stretch mine[V];
+    Vec<V> A[L], B[L], P[L], E[L];  // gates, states before each row, what enters each row from its output
+    Stretch<V> mine = nothing<V>();
+    const auto scan = [&](auto plain) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) mine[v] = Stretch{1.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      if (i < n) {
-        float x[V], g[V];
-        words.read(stage, 0, row, i, x);
-        words.read(stage, 1, row, i, g);
-#pragma unroll
-        for (int v = 0; v < V; ++v) gate_of(g[v] + bias[v], A[i][v], B[i][v]);
-        if (first >> i & 1) {
-          const float* const h0 = a.state0 ? a.state0 + sequence_of(a, row + i).index * a.channels + c : nullptr;
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            P[i][v] = h0 ? h0[v] : 0.f;
-            mine[v] = Stretch{-1.f, fmaf(A[i][v], P[i][v], B[i][v] * x[v])};
+      for (int i = 0; i < L; ++i) {
+        if (plain || i < n) {
+          gate_of(words.read(kG, gs, a.g_stride, i) + bias, A[i], B[i]);
+          const Vec<V> in_x = B[i] * words.read(kX + stage, xs, a.x_stride, i);
+          if (!plain && (at.first >> i & 1)) {
+            P[i] = a.state0 ? load_floats<V>(a.state0 + index_of(a, row + i) * a.channels + c) : all_of<V>(0.f);
+            mine = Stretch<V>{all_of<V>(-1.f), fma(A[i], P[i], in_x)};
+          } else {
+            const bool cut = !plain && mine.A.x < 0.f;
+            mine = Stretch<V>{cut ? mine.A : mine.A * A[i], fma(A[i], mine.H, in_x)};
           }
         } else {
-#pragma unroll
-          for (int v = 0; v < V; ++v)
-            mine[v] = Stretch{mine[v].A < 0.f ? -1.f : mine[v].A * A[i][v], fmaf(A[i][v], mine[v].H, B[i][v] * x[v])};
+          A[i] = all_of<V>(1.f), B[i] = all_of<V>(0.f);
         }
-      } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) A[i][v] = 1.f, B[i][v] = 0.f;
       }
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) states[stage][warp][lane][v] = mine[v];
+    };
+    if (within) scan(std::true_type{});
+    else scan(std::false_type{});
+    fetch_inputs(round + 1);
+    states[stage][warp][lane] = mine;
     __syncthreads();
-    float h[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      h[v] = entered[v];
-      for (int w = 0; w < warp; ++w) h[v] = apply(states[stage][w][lane][v], h[v]);
-    }
+    for (int w = 0; w < warp; ++w) h = apply(states[stage][w][lane], h);
+    words.wait();
     T* dz = static_cast<T*>(a.dz) + row * a.dz_stride + c;
+    // forward from row to row; then back, what flows to the rows before: d -> A (E + d), nothing across the beginning
+    // of a sequence
+    mine = nothing<V>();
+    const auto through = [&](auto plain) {
 #pragma unroll
-    for (int i = 0; i < L; ++i) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) E[i][v] = 0.f;
-      if (i >= n) continue;
-      float x[V], dy[V];
-      words.read(stage, 0, row, i, x);
-      words.read(stage, 2, row, i, dy);
-      const bool start = first >> i & 1;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        P[i][v] = start ? P[i][v] : h[v];
-        h[v] = fmaf(A[i][v], P[i][v], B[i][v] * x[v]);
-        E[i][v] = dy[v];
-      }
-      if (kGate) {
-        float z[V];
-        words.read(stage, kStreams - 1, row, i, z);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float s = sigmoid(z[v]);
-          E[i][v] = dy[v] * (z[v] * s);
-          z[v] = dy[v] * h[v] * (s * fmaf(z[v], 1.f - s, 1.f));
+      for (int i = 0; i < L; ++i) {
+        E[i] = all_of<V>(0.f);
+        if (!plain && i >= n) continue;
+        const Vec<V> dy = words.read(kDy, dys, a.dy_stride, i);
+        const bool start = !plain && (at.first >> i & 1);
+        P[i] = start ? P[i] : h;
+        h = fma(A[i], P[i], B[i] * words.read(kX + stage, xs, a.x_stride, i));
+        E[i] = dy;
+        if (kGate) {
+          const Vec<V> z = words.read(kZ, zs, a.z_stride, i), s = sigmoid(z), ds = dy * s;
+          E[i] = ds * z;
+          // dy h s (1 + z (1 - s))
+          const Vec<V> slope = fma(z, fma(s, all_of<V>(-1.f), all_of<V>(1.f)), all_of<V>(1.f));
+          if (a.dz && on) store_word<T, V>(dz + i * a.dz_stride, (ds * h) * slope);
         }
-        if (a.dz && on) store_word<T, V>(dz + i * a.dz_stride, z);
+        if (!plain && (at.last >> i & 1) && a.dstate)
+          E[i] = E[i] + load_floats<V>(a.dstate + index_of(a, row + i) * a.channels + c);
       }
-      if ((last >> i & 1) && a.dstate) {
-        const float* const from = a.dstate + sequence_of(a, row + i).index * a.channels + c;
 #pragma unroll
-        for (int v = 0; v < V; ++v) E[i][v] += from[v];
+      for (int i = L - 1; i >= 0; --i) {
+        if (!plain && i >= n) continue;
+        const bool start = !plain && (at.first >> i & 1), cut = !plain && mine.A.x < 0.f;
+        mine = start ? Stretch<V>{all_of<V>(-1.f), all_of<V>(0.f)}
+                     : Stretch<V>{cut ? mine.A : mine.A * A[i], A[i] * (E[i] + mine.H)};
       }
-    }
-    // what flows to the rows before: d -> A (E + d), nothing across the beginning of a sequence
-#pragma unroll
-    for (int v = 0; v < V; ++v) mine[v] = Stretch{1.f, 0.f};
-#pragma unroll
-    for (int i = L - 1; i >= 0; --i) {
-      if (i >= n) continue;
-      const bool start = first >> i & 1;
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        mine[v] = start ? Stretch{-1.f, 0.f}
-                        : Stretch{mine[v].A < 0.f ? -1.f : mine[v].A * A[i][v], A[i][v] * (E[i][v] + mine[v].H)};
-    }
-    float d[V];
-    exchange(shared, stage, kWarps - 1 - warp, rank, blocks, mine, carry, d);
+    };
+    if (within) through(std::true_type{});
+    else through(std::false_type{});
+    fetch_outputs(round + 1);
+    Vec<V> d = exchange(shared, stage, kWarps - 1 - warp, rank, blocks, mine, carry);
     T* dx = static_cast<T*>(a.dx) + row * a.dx_stride + c;
     T* dg = static_cast<T*>(a.dg) + row * a.dg_stride + c;
+    const auto emit = [&](auto plain) {
 #pragma unroll
-    for (int i = L - 1; i >= 0; --i) {
-      if (i >= n) continue;
-      float x[V], out[V];
-      words.read(stage, 0, row, i, x);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        d[v] += E[i][v];
-        out[v] = B[i][v] * d[v];
-        x[v] = out[v] * A[i][v] * (P[i][v] - x[v]);
-        dbias[v] += x[v];
-        d[v] *= A[i][v];
-      }
-      if (a.dx && on) store_word<T, V>(dx + i * a.dx_stride, out);
-      if (a.dg && on) store_word<T, V>(dg + i * a.dg_stride, x);
-      if (first >> i & 1) {
-        if (a.dstate0 && on) {
-          float* const to = a.dstate0 + sequence_of(a, row + i).index * a.channels + c;
-#pragma unroll
-          for (int v = 0; v < V; ++v) to[v] = d[v];
+      for (int i = L - 1; i >= 0; --i) {
+        if (!plain && i >= n) continue;
+        d = d + E[i];
+        const Vec<V> out = B[i] * d;
+        const Vec<V> way = fma(words.read(kX + stage, xs, a.x_stride, i), all_of<V>(-1.f), P[i]);
+        const Vec<V> gate = (out * A[i]) * way;
+        dbias = dbias + gate;
+        d = d * A[i];
+        if (a.dx && on) store_word<T, V>(dx + i * a.dx_stride, out);
+        if (a.dg && on) store_word<T, V>(dg + i * a.dg_stride, gate);
+        if (!plain && (at.first >> i & 1)) {
+          if (a.dstate0 && on) store_floats(a.dstate0 + index_of(a, row + i) * a.channels + c, d);
+          d = all_of<V>(0.f);
         }
-#pragma unroll
-        for (int v = 0; v < V; ++v) d[v] = 0.f;
       }
-    }
-    words.fetch(stage, row_of(round + 2), rows_at(round + 2), on);
+    };
+    if (within) emit(std::true_type{});
+    else emit(std::false_type{});
   }
   if (!a.sums) return;
   __syncthreads();
-#pragma unroll
-  for (int v = 0; v < V; ++v) states[0][warp][lane][v].H = dbias[v];
+  states[0][warp][lane].H = dbias;
   __syncthreads();
   if (warp == 0 && on) {
-    float* const to = a.sums + ((long long)blockIdx.y * blocks + rank) * a.channels + c;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float s = 0.f;
-      for (int w = 0; w < kWarps; ++w) s += states[0][w][lane][v].H;
-      to[v] = s;
-    }
+    Vec<V> s = all_of<V>(0.f);
+    for (int w = 0; w < kWarps; ++w) s = s + states[0][w][lane].H;
+    store_floats(a.sums + ((long long)blockIdx.y * blocks + rank) * a.channels + c, s);
   }
 }
 
@@ -548,81 +616,120 @@ __global__ void __launch_bounds__(128) recurrence_step_kernel(const RecArgs a) {
   const int c = (blockIdx.x * 128 + threadIdx.x) * V;
   if (c >= a.channels) return;
   for (long long s = blockIdx.y; s < a.sequences; s += gridDim.y) {
-    float x[V], g[V], z[V], out[V];
-    unpack<T, V>(load_word<T, V>(static_cast<const T*>(a.x) + s * a.x_stride + c), x);
-    unpack<T, V>(load_word<T, V>(static_cast<const T*>(a.g) + s * a.g_stride + c), g);
-    if (kGate) unpack<T, V>(load_word<T, V>(static_cast<const T*>(a.z) + s * a.z_stride + c), z);
+    const Vec<V> x = unpack<T, V>(load_word<T, V>(static_cast<const T*>(a.x) + s * a.x_stride + c));
+    const Vec<V> g = unpack<T, V>(load_word<T, V>(static_cast<const T*>(a.g) + s * a.g_stride + c));
     float* const state = a.state + s * a.channels + c;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float fa, fb;
-      gate_of(g[v] + (a.bias ? a.bias[c + v] : 0.f), fa, fb);
-      const float h = fmaf(fa, state[v], fb * x[v]);
-      state[v] = h;
-      out[v] = kGate ? h * (z[v] * sigmoid(z[v])) : h;
+    Vec<V> fa, fb;
+    gate_of(a.bias ? g + load_floats<V>(a.bias + c) : g, fa, fb);
+    const Vec<V> h = fma(fa, load_floats<V>(state), fb * x);
+    Vec<V> out = h;
+    if (kGate) {
+      const Vec<V> z = unpack<T, V>(load_word<T, V>(static_cast<const T*>(a.z) + s * a.z_stride + c));
+      out = (h * z) * sigmoid(z);
     }
+    store_floats(state, h);
     store_word<T, V>(static_cast<T*>(a.y) + s * a.y_stride + c, out);
   }
 }
 
 // ---- host -------------------------------------------------------------------------------------------
 struct Division {
-  int tiles, segments, cluster;  // of channels; of sequences; blocks that share a segment's rows
-  long long per_segment, checkpoints;
+  int tiles, segments;  // of channels; of sequences
+  long long rows, per_segment, checkpoints;  // of a segment
 };
 
-// Blocks for the whole GPU, two to an SM: over channels, then over sequences of known borders, then over time.
-Division split_of(const fbfftconv_recurrence_desc& d, int V) {
+// Blocks over channels, then over sequences of known borders, two to an SM; what is left goes to clusters over time.
+Division division_of(const fbfftconv_recurrence_desc& d, int V) {
   Division s{};
   s.tiles = (d.channels + 32 * V - 1) / (32 * V);
-  const long long want = 2ll * sm_count();
-  long long segments = d.offsets ? 1 : want / s.tiles;
+  long long segments = d.offsets ? 1 : 2ll * sm_count() / s.tiles;
   if (segments > d.sequences) segments = d.sequences;
   if (segments < 1) segments = 1;
   s.per_segment = d.sequences > 0 ? (d.sequences + segments - 1) / segments : 1;
   s.segments = (int)(d.sequences > 0 ? (d.sequences + s.per_segment - 1) / s.per_segment : 1);
-  const long long rows = d.offsets ? d.rows : s.per_segment * d.length;
-  s.checkpoints = (rows + kCheckpoint - 1) / kCheckpoint;
-  s.cluster = 1;
-  while (s.cluster < kMostCluster && (long long)s.tiles * s.segments * s.cluster * 2 <= want &&
-         (long long)s.cluster * 2 * kCheckpoint <= rows)
-    s.cluster *= 2;
+  s.rows = d.offsets ? d.rows : s.per_segment * d.length;
+  s.checkpoints = (s.rows + kCheckpoint - 1) / kCheckpoint;
   return s;
 }
 
-template <typename K>
-cudaError_t launch_split(K kernel, const RecArgs& a, const Division& s, size_t smem, cudaStream_t stream) {
-  const cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), (int)smem);
-  if (e != cudaSuccess) return e;
+cudaLaunchConfig_t config_of(const Division& s, int cluster, size_t smem, cudaStream_t stream, cudaLaunchAttribute (&attrs)[2]) {
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(s.tiles * s.cluster, s.segments);
+  config.gridDim = dim3(s.tiles * cluster, s.segments);
   config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
-  cudaLaunchAttribute attrs[2]{};
   attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attrs[0].val.programmaticStreamSerializationAllowed = 1;
   attrs[1].id = cudaLaunchAttributeClusterDimension;
-  attrs[1].val.clusterDim.x = s.cluster, attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+  attrs[1].val.clusterDim.x = cluster, attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
   config.attrs = attrs;
-  config.numAttrs = s.cluster > 1 ? 2 : 1;
-  const cudaError_t r = cudaLaunchKernelEx(&config, kernel, a);
-  if (r != cudaSuccess) cudaGetLastError();
-  return r;
+  config.numAttrs = cluster > 1 ? 2 : 1;
+  return config;
+}
+
+// Clusters of a size that the current GPU holds at once, asked once for each kernel.
+int resident_clusters(const void* kernel, int cluster, size_t smem) {
+  struct Known {
+    const void* kernel;
+    int device, clusters[kMostCluster + 1];
+  };
+  static Known known[64];
+  static std::mutex lock;
+  const std::lock_guard<std::mutex> hold(lock);
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return 0;
+  Known* k = known;
+  while (k < known + 63 && k->kernel && (k->kernel != kernel || k->device != device)) ++k;
+  if (k->kernel != kernel || k->device != device) *k = Known{kernel, device, {}};
+  if (k->clusters[cluster] == 0) {
+    Division one{};
+    one.tiles = one.segments = 1;
+    cudaLaunchAttribute attrs[2]{};
+    const cudaLaunchConfig_t config = config_of(one, cluster, smem, nullptr, attrs);
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &config) != cudaSuccess) cudaGetLastError(), n = 0;
+    k->clusters[cluster] = n > 0 ? n : -1;
+  }
+  return k->clusters[cluster];
+}
+
+// The widest cluster of which the GPU holds as many at once as there are: a second wave of them would double the time
+// (16 clusters of 16 blocks: 14 are held, and 131072 x 1024 took 1214 us; of NN blocks NNN us).  A block has at least
+// one round of rows.
+template <typename K>
+cudaError_t launch_divided(K kernel, RecArgs a, const Division& s, int tile_rows, size_t smem, int* parts, cudaStream_t stream) {
+  const void* const pointer = reinterpret_cast<const void*>(kernel);
+  cudaError_t e = ensure_dynamic_smem(pointer, (int)smem);
+  const long long groups = (long long)s.tiles * s.segments, tiles = (s.rows + tile_rows - 1) / tile_rows;
+  a.cluster = 1;
+  if (e == cudaSuccess && tiles > 1 && groups < 2ll * sm_count()) {
+    e = cudaFuncSetAttribute(pointer, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    for (int c = (int)(tiles < kMostCluster ? tiles : kMostCluster); c > 1 && a.cluster == 1; --c)
+      if (resident_clusters(pointer, c, smem) >= groups) a.cluster = c;
+  }
+  if (e != cudaSuccess) return e;
+  if (parts) *parts = s.segments * a.cluster;
+  cudaLaunchAttribute attrs[2]{};
+  const cudaLaunchConfig_t config = config_of(s, a.cluster, smem, stream, attrs);
+  e = cudaLaunchKernelEx(&config, kernel, a);
+  if (e != cudaSuccess) cudaGetLastError();  // returned here; the next launch must not report it again
+  return e;
 }
 
 template <typename T, int V>
 cudaError_t forward(const RecArgs& a, const Division& s, cudaStream_t stream) {
-  const size_t row = sizeof(T) * V == 4 ? 2ull * kForwardRows * kThreads * 4 : 0;
-  return a.z ? launch_split(recurrence_forward_kernel<T, V, true>, a, s, 3 * row, stream)
-             : launch_split(recurrence_forward_kernel<T, V, false>, a, s, 2 * row, stream);
+  constexpr size_t slot = sizeof(T) * V == 4 ? kForwardRows * kThreads * 4 : 0;
+  constexpr int tile = kWarps * kForwardRows;
+  return a.z ? launch_divided(recurrence_forward_kernel<T, V, true>, a, s, tile, 3 * slot, nullptr, stream)
+             : launch_divided(recurrence_forward_kernel<T, V, false>, a, s, tile, 2 * slot, nullptr, stream);
 }
 
 template <typename T, int V>
-cudaError_t backward(const RecArgs& a, const Division& s, cudaStream_t stream) {
-  const size_t row = sizeof(T) * V == 4 ? 2ull * kBackwardRows * kThreads * 4 : 0;
-  return a.z ? launch_split(recurrence_backward_kernel<T, V, true>, a, s, 4 * row, stream)
-             : launch_split(recurrence_backward_kernel<T, V, false>, a, s, 3 * row, stream);
+cudaError_t backward(const RecArgs& a, const Division& s, int* parts, cudaStream_t stream) {
+  constexpr size_t slot = sizeof(T) * V == 4 ? kBackwardRows * kThreads * 4 : 0;
+  constexpr int tile = kWarps * kBackwardRows;
+  return a.z ? launch_divided(recurrence_backward_kernel<T, V, true>, a, s, tile, 5 * slot, parts, stream)
+             : launch_divided(recurrence_backward_kernel<T, V, false>, a, s, tile, 4 * slot, parts, stream);
 }
 
 template <typename T, int V>
@@ -690,9 +797,9 @@ RecArgs common_args(const fbfftconv_recurrence_desc& d) {
 
 // 16-bit channels travel in pairs or alone, which changes how many blocks share the channels; what is kept between the
 // passes must not depend on that.
-Division split_for(const fbfftconv_recurrence_desc& d, bool pairs) {
+Division division_for(const fbfftconv_recurrence_desc& d, bool pairs) {
   const int V = d.type == FBFFTCONV_FLOAT32 ? 1 : 2;
-  Division s = split_of(d, V);
+  Division s = division_of(d, V);
   if (V == 2 && !pairs) s.tiles = (d.channels + 31) / 32;
   return s;
 }
@@ -709,7 +816,7 @@ size_t fbfftconv_recurrence_checkpoint_bytes(const fbfftconv_recurrence_desc* de
   int device;
   if (resolve_device(desc->device, &device) != FBFFTCONV_OK) return 0;
   const OnDevice on(device);
-  const Division s = split_for(*desc, true);
+  const Division s = division_for(*desc, true);
   return (size_t)(s.segments * s.checkpoints) * desc->channels * sizeof(float);
 }
 
@@ -718,8 +825,8 @@ size_t fbfftconv_recurrence_workspace_bytes(const fbfftconv_recurrence_desc* des
   int device;
   if (resolve_device(desc->device, &device) != FBFFTCONV_OK) return 0;
   const OnDevice on(device);
-  const Division s = split_for(*desc, true);
-  return (size_t)s.segments * s.cluster * desc->channels * sizeof(float);
+  const Division s = division_for(*desc, true);
+  return (size_t)s.segments * kMostCluster * desc->channels * sizeof(float);
 }
 
 int fbfftconv_recurrence(const fbfftconv_recurrence_desc* desc, const void* x, const void* g, const void* z,
@@ -741,9 +848,9 @@ int fbfftconv_recurrence(const fbfftconv_recurrence_desc* desc, const void* x, c
   if (d.sequences == 0) return FBFFTCONV_OK;
   const OnDevice on(device);
   if (on.error() != cudaSuccess) return op_cuda_fail(on.error(), "cudaSetDevice");
-  const Division s = split_for(d, pairs);
+  const Division s = division_for(d, pairs);
   a.x = x, a.g = g, a.z = z, a.bias = bias, a.state0 = state0, a.y = y, a.state = state, a.checkpoints = checkpoints;
-  a.per_segment = s.per_segment, a.checkpoints_per_segment = s.checkpoints, a.cluster = s.cluster;
+  a.per_segment = s.per_segment, a.checkpoints_per_segment = s.checkpoints;
   count_launch();
 #define FORWARD(T, V) forward<T, V>(a, s, static_cast<cudaStream_t>(stream))
   const cudaError_t e = BY_TYPE(FORWARD);
@@ -776,18 +883,18 @@ int fbfftconv_recurrence_backward(const fbfftconv_recurrence_desc* desc, const v
   OP_TRY(check_rec_pointers(rows, floats, d, device, &pairs));
   const OnDevice on(device);
   if (on.error() != cudaSuccess) return op_cuda_fail(on.error(), "cudaSetDevice");
-  const Division s = split_for(d, pairs);
-  const int parts = d.sequences > 0 ? s.segments * s.cluster : 0;
-  if (grad_bias && workspace_bytes < (size_t)parts * d.channels * sizeof(float))
+  const Division s = division_for(d, pairs);
+  int parts = 0;
+  if (grad_bias && d.sequences > 0 && workspace_bytes < (size_t)s.segments * kMostCluster * d.channels * sizeof(float))
     return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "the workspace is smaller than fbfftconv_recurrence_workspace_bytes");
   const cudaStream_t cuda_stream = static_cast<cudaStream_t>(stream);
   if (d.sequences > 0) {
     a.x = x, a.g = g, a.z = z, a.bias = bias, a.state0 = state0, a.checkpoints = const_cast<float*>(checkpoints);
     a.dy = grad_y, a.dstate = grad_state, a.dx = grad_x, a.dg = grad_g, a.dz = grad_z, a.dstate0 = grad_state0;
     a.sums = grad_bias ? static_cast<float*>(workspace) : nullptr;
-    a.per_segment = s.per_segment, a.checkpoints_per_segment = s.checkpoints, a.cluster = s.cluster;
+    a.per_segment = s.per_segment, a.checkpoints_per_segment = s.checkpoints;
     count_launch();
-#define BACKWARD(T, V) backward<T, V>(a, s, cuda_stream)
+#define BACKWARD(T, V) backward<T, V>(a, s, &parts, cuda_stream)
     const cudaError_t e = BY_TYPE(BACKWARD);
 #undef BACKWARD
     if (e != cudaSuccess) return op_cuda_fail(e, "recurrence, backward");

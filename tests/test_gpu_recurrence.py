@@ -5,7 +5,7 @@ carries |g| u, exp and quotient a few u).  a + (1 - a) = 1 to u / 2, so an error
 |x - h|, in all at most 2 eps M with M the largest |x|, |h|; rounding and joining of stretches adds some 6 u M a row for
 as many rows as the memory reaches, N = min(length, 1 / min(1 - a)).  D sums |e| with weights a: S_t = |e_t| + a_{t+1}
 S_{t+1}, within S (6 u N + 4 eps).  Products add their factors' errors.  Below the normal numbers (|g| > 87) the smaller of a and 1 - a
-is good to 2^-126 alone, which is what eps a (1 - a) gains there.  16-bit outputs add half a step."""
+is good to 2^-126 alone (`lost`), which is added to eps times it there.  16-bit outputs add half a step."""
 import pytest
 import torch
 
@@ -48,7 +48,8 @@ def reference(x, g, z, bias, offsets, state, dy=None, dstate=None):
             h[t] = cur
         final[i] = cur
         eps[rows] = eps[rows].amax(0)
-    tol_h = largest * (2 * eps + 6 * U * reach)
+    lost = 2.0 ** -126 * (g.abs() > 87)
+    tol_h = largest * (2 * eps + 6 * U * reach + lost * reach)
     out = {}
     sz = torch.sigmoid(z) if z is not None else None
     soft = (z.abs() + 6) * 2.0 ** -22 if z is not None else None
@@ -75,9 +76,8 @@ def reference(x, g, z, bias, offsets, state, dy=None, dstate=None):
             flow, sums, slack = a[t] * D[t], a[t] * S[t], a[t] * G[t]
         d0[i] = flow
         first = offsets[i]
-        s0[i] = a[first] * (S[first] * (6 * U * reach[first] + 6 * eps[first]) + G[first])
+        s0[i] = a[first] * (S[first] * (6 * U * reach[first] + 6 * eps[first]) + G[first]) + lost[first] * S[first]
     tol_D = S * (6 * U * reach + 4 * eps) + G
-    lost = 2.0 ** -126 * (g.abs() > 87)
     out["dx"] = (b * D, b * (tol_D + S * 2 * eps) + lost * S)
     dg = D * (prev - x) * a * b
     tol_g = a * b * ((tol_D + S * 6 * eps) * 2 * largest + S * (tol_h + 4 * U * largest)) + lost * S * 2 * largest

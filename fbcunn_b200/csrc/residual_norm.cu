@@ -21,6 +21,7 @@ namespace fbfft {
 namespace {
 
 constexpr int kMostChannels = 16384;
+constexpr long long kMostRows = 1ll << 30, kMostStride = 1ll << 30;  // rows and strides are 32 bits wide in the kernels
 
 struct NormArgs {
   const void* u;
@@ -41,13 +42,17 @@ struct NormArgs {
   void* dgate;
   float* sums;        // a worker's sums: [kind][worker][channel]
   float* gate_sums;   // [worker][channel], or null: a worker has whole gate rows to itself
-  long long rows, u_stride, r_stride, gate_stride, per_gate;  // per_gate: rows that share a gate row
+  int rows, u_stride, r_stride, gate_stride, per_gate;  // per_gate: rows that share a gate row
   int channels, lanes, post, pre, gate_kind;
   int splits;         // workers to a gate row, where rows share it
   int stages;         // rows under way in the ring
   bool vectors;
   float eps, alpha, beta;
 };
+
+template <typename E> __device__ __forceinline__ E* row_of(const void* p, int row, int stride) {
+  return static_cast<E*>(const_cast<void*>(p)) + (long long)row * stride;
+}
 
 // A thread's columns of a row: chunks of neighbours one vector wide, or single ones a row's lanes apart where a
 // pointer, a stride or the width does not allow vectors.
@@ -177,32 +182,43 @@ struct Ring {
   }
 };
 
-// Sums over the lanes of a row, for everyone.  Two exchanges in turn use the two halves of `part`: a warp that is
-// through with one cannot reach the next but one before all have left the first.
+// Sums over the lanes of a row, for everyone: shuffles within a warp, then every thread adds the warps' sums in their
+// order.  Two exchanges in turn use the two halves of `part`: a warp that is through with one cannot reach the next but
+// one before all have left the first.  What lies behind the last warp's sums must be zero.
 struct RowSums {
-  float2* part;  // [2][32]
+  float (*part)[2][32];
   int lanes, turn;
-  __device__ __forceinline__ float2 operator()(float a, float b) {
+  template <int N>
+  __device__ __forceinline__ void operator()(float (&x)[N]) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      a += __shfl_xor_sync(0xffffffffu, a, o);
-      b += __shfl_xor_sync(0xffffffffu, b, o);
-    }
-    if (lanes <= 32) return make_float2(a, b);
-    float2* const mine = part + 32 * turn;
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) x[k] += __shfl_xor_sync(0xffffffffu, x[k], o);
+    if (lanes <= 32) return;
+    float(*const mine)[32] = part[turn];
     turn ^= 1;
-    if ((threadIdx.x & 31) == 0) mine[threadIdx.x >> 5] = make_float2(a, b);
-    __syncthreads();
-    const float2 other = (threadIdx.x & 31) < lanes / 32 ? mine[threadIdx.x & 31] : make_float2(0.f, 0.f);
-    a = other.x, b = other.y;
+    if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      a += __shfl_xor_sync(0xffffffffu, a, o);
-      b += __shfl_xor_sync(0xffffffffu, b, o);
+      for (int k = 0; k < N; ++k) mine[k][threadIdx.x >> 5] = x[k];
     }
-    return make_float2(a, b);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      float s = 0.f;
+      for (int w = 0; w < lanes / 32; w += 4) {
+        const float4 q = *reinterpret_cast<const float4*>(&mine[k][w]);
+        s += (q.x + q.y) + (q.z + q.w);
+      }
+      x[k] = s;
+    }
   }
 };
+
+__device__ __forceinline__ void clear_sums(float (*part)[2][32]) {
+  if (threadIdx.x < 128) (&part[0][0][0])[threadIdx.x] = 0.f;
+  for (int i = threadIdx.x + blockDim.x; i < 128; i += blockDim.x) (&part[0][0][0])[i] = 0.f;
+  __syncthreads();
+}
 
 // x becomes x - mean; returns (mean, 1 / deviation).
 template <int C, int kVec, bool kRing>
@@ -213,42 +229,59 @@ __device__ __forceinline__ float2 normalise(float (&x)[C], int kind, const Colum
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < C; ++i) s += x[i];
-    mean = sums(s, 0.f).x * per;
+    float one[1] = {s};
+    sums(one);
+    mean = one[0] * per;
 #pragma unroll
     for (int i = 0; i < C; ++i) x[i] = c.has(i) ? x[i] - mean : 0.f;
   }
   float q = 0.f;
 #pragma unroll
   for (int i = 0; i < C; ++i) q = fmaf(x[i], x[i], q);
-  const float rstd = 1.f / sqrtf(fmaf(sums(q, 0.f).x, per, eps));
-  return make_float2(mean, rstd);
+  float one[1] = {q};
+  sums(one);
+  return make_float2(mean, 1.f / sqrtf(fmaf(one[0], per, eps)));
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + __expf(-x)); }
+__device__ __forceinline__ float sigmoid(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-x)));
+  return r;
+}
+
+// y = act(y), in one loop for each kind of gate
+template <int C> __device__ __forceinline__ void activate(float (&y)[C], int kind) {
+  if (kind != FBFFTCONV_GATE_SIGMOID) return;
+#pragma unroll
+  for (int i = 0; i < C; ++i) y[i] = sigmoid(y[i]);
+}
 
 template <typename T, int C> constexpr int pieces_of() { return C * (int)sizeof(T) / 16; }
 
 template <typename T, typename TR, int C, int kThreads, bool kRing>
-__global__ void __launch_bounds__(kThreads) norm_forward_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 3 : kThreads <= 320 ? 2 : 1) norm_forward_kernel(const NormArgs a) {
   constexpr int kVec = std::is_same_v<T, float> ? 4 : 8;
   constexpr int kT = pieces_of<T, C>(), kTR = pieces_of<TR, C>();
-  __shared__ float2 part[64];
+  __shared__ __align__(16) float part[2][2][32];
   extern __shared__ __align__(16) char staged[];
+  clear_sums(part);
   grid_dependency_wait();
   const int slot = threadIdx.x / a.lanes, slots = blockDim.x / a.lanes;
   const Columns<C, kVec, kRing> c((int)threadIdx.x % a.lanes, a.lanes, a.channels, a.vectors);
   RowSums sums{part, a.lanes, 0};
-  const long long stride = (long long)gridDim.x * slots;
+  const int stride = gridDim.x * slots;
   const Ring<C, kVec, kRing> ring{staged + 16 * threadIdx.x, (2 * kT + kTR) * 16 * (int)blockDim.x, 16 * (int)blockDim.x, a.stages};
-  const auto fetch = [&](long long row, int stage) {
+  const auto gate_row_of = [&](int row) { return a.per_gate == 1 ? row : row / a.per_gate; };
+  const auto fetch = [&](int row, int stage) {
     if (row < a.rows) {
-      ring.fetch(stage, 0, static_cast<const TR*>(a.r) + row * a.r_stride, c);
-      if (a.u) ring.fetch(stage, kTR, static_cast<const T*>(a.u) + row * a.u_stride, c);
-      if (a.gate_kind) ring.fetch(stage, kTR + kT, static_cast<const T*>(a.gate) + row / a.per_gate * a.gate_stride, c);
+      const int gate_row = gate_row_of(row);
+      ring.fetch(stage, 0, row_of<const TR>(a.r, row, a.r_stride), c);
+      if (a.u) ring.fetch(stage, kTR, row_of<const T>(a.u, row, a.u_stride), c);
+      if (a.gate_kind) ring.fetch(stage, kTR + kT, row_of<const T>(a.gate, gate_row, a.gate_stride), c);
     }
     ring.commit();
   };
-  long long row = (long long)blockIdx.x * slots + slot;
+  int row = blockIdx.x * slots + slot;
   if (kRing)
     for (int k = 0; k < a.stages; ++k) fetch(row + k * stride, k);
   for (int stage = 0; row < a.rows; row += stride, stage = stage + 1 < a.stages ? stage + 1 : 0) {
@@ -258,20 +291,20 @@ __global__ void __launch_bounds__(kThreads) norm_forward_kernel(const NormArgs a
       if (a.u) ring.template read<T>(stage, kTR, c, x);
       ring.template read<TR>(stage, 0, c, r);
     } else {
-      if (a.u) load_row(static_cast<const T*>(a.u) + row * a.u_stride, c, x);
-      load_row(static_cast<const TR*>(a.r) + row * a.r_stride, c, r);
+      if (a.u) load_row(row_of<const T>(a.u, row, a.u_stride), c, x);
+      load_row(row_of<const TR>(a.r, row, a.r_stride), c, r);
     }
     float2 first = make_float2(0.f, 1.f), second = first;
     if (a.u) {
       float g[C];
       if (a.gate_kind) {
         if (kRing) ring.template read<T>(stage, kTR + kT, c, g);
-        else load_row(static_cast<const T*>(a.gate) + row / a.per_gate * a.gate_stride, c, g);
+        else load_row(row_of<const T>(a.gate, gate_row_of(row), a.gate_stride), c, g);
       }
       if (kRing) fetch(row + a.stages * stride, stage);
       if (a.post) {
+        load_row(a.w1, c, w);  // on its way during the sums
         first = normalise(x, a.post, c, sums, a.eps);
-        load_row(a.w1, c, w);
 #pragma unroll
         for (int i = 0; i < C; ++i) x[i] *= first.y * w[i];
         if (a.b1) {
@@ -281,18 +314,20 @@ __global__ void __launch_bounds__(kThreads) norm_forward_kernel(const NormArgs a
         }
       }
       if (a.gate_kind) {
+        activate(g, a.gate_kind);
 #pragma unroll
-        for (int i = 0; i < C; ++i) x[i] *= a.gate_kind == FBFFTCONV_GATE_SIGMOID ? sigmoid(g[i]) : g[i];
+        for (int i = 0; i < C; ++i) x[i] *= g[i];
       }
 #pragma unroll
       for (int i = 0; i < C; ++i) r[i] = fmaf(a.beta, x[i], a.alpha * r[i]);
-      store_row(static_cast<TR*>(a.r_out) + row * a.channels, c, r);
-    } else if (kRing) {
-      fetch(row + a.stages * stride, stage);
+      if (a.pre) load_row(a.w2, c, w);
+      store_row(row_of<TR>(a.r_out, row, a.channels), c, r);
+    } else {
+      if (kRing) fetch(row + a.stages * stride, stage);
+      load_row(a.w2, c, w);
     }
     if (a.pre) {
       second = normalise(r, a.pre, c, sums, a.eps);
-      load_row(a.w2, c, w);
 #pragma unroll
       for (int i = 0; i < C; ++i) r[i] *= second.y * w[i];
       if (a.b2) {
@@ -300,7 +335,7 @@ __global__ void __launch_bounds__(kThreads) norm_forward_kernel(const NormArgs a
 #pragma unroll
         for (int i = 0; i < C; ++i) r[i] += b[i];
       }
-      store_row(static_cast<T*>(a.v) + row * a.channels, c, r);
+      store_row(row_of<T>(a.v, row, a.channels), c, r);
     }
     if (a.stats && c.lane == 0) a.stats[row] = make_float4(first.x, first.y, second.x, second.y);
   }
@@ -312,8 +347,9 @@ template <typename T, typename TR, int C, int kThreads, bool kAll, bool kRing>
 __global__ void __launch_bounds__(kThreads) norm_backward_kernel(const NormArgs a) {
   constexpr int kVec = std::is_same_v<T, float> ? 4 : 8;
   constexpr int kT = pieces_of<T, C>(), kTR = pieces_of<TR, C>();
-  __shared__ float2 part[64];
+  __shared__ __align__(16) float part[2][2][32];
   extern __shared__ __align__(16) char staged[];
+  clear_sums(part);
   grid_dependency_wait();
   const int slots = blockDim.x / a.lanes;
   const int worker = blockIdx.x * slots + threadIdx.x / a.lanes, workers = gridDim.x * slots;
@@ -322,18 +358,18 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(const NormArgs 
   const float per = 1.f / (float)a.channels;
   const bool shared_gate = kAll && a.gate_kind && a.per_gate > 1;
   // without shared gate rows all rows are one stretch, dealt out in turn; else `splits` workers deal out a gate row's
-  const long long stretch = shared_gate ? a.per_gate : a.rows, stretches = a.rows / (stretch > 0 ? stretch : 1);
+  const int stretch = shared_gate ? a.per_gate : a.rows, stretches = a.rows / stretch;
   const int splits = shared_gate ? a.splits : workers;
   const Ring<C, kVec, kRing> ring{staged + 16 * threadIdx.x, (3 * kT + 2 * kTR) * 16 * (int)blockDim.x, 16 * (int)blockDim.x, a.stages};
   enum { kR = 0, kDr = kTR, kU = 2 * kTR, kGate = kU + kT, kDv = kGate + kT };  // pieces of a stage
   const bool need_u = a.u && (a.post || a.gate_kind || a.pre);
-  const auto fetch = [&](long long row, long long end, int stage) {
+  const auto fetch = [&](int row, int end, int gate_row, int stage) {
     if (row < end) {
-      if (a.pre) ring.fetch(stage, kR, static_cast<const TR*>(a.r) + row * a.r_stride, c);
-      if (a.dr_out) ring.fetch(stage, kDr, static_cast<const TR*>(a.dr_out) + row * a.channels, c);
-      if (need_u) ring.fetch(stage, kU, static_cast<const T*>(a.u) + row * a.u_stride, c);
-      if (a.gate_kind) ring.fetch(stage, kGate, static_cast<const T*>(a.gate) + row / a.per_gate * a.gate_stride, c);
-      if (a.pre) ring.fetch(stage, kDv, static_cast<const T*>(a.dv) + row * a.channels, c);
+      if (a.pre) ring.fetch(stage, kR, row_of<const TR>(a.r, row, a.r_stride), c);
+      if (a.dr_out) ring.fetch(stage, kDr, row_of<const TR>(a.dr_out, row, a.channels), c);
+      if (need_u) ring.fetch(stage, kU, row_of<const T>(a.u, row, a.u_stride), c);
+      if (a.gate_kind) ring.fetch(stage, kGate, row_of<const T>(a.gate, gate_row, a.gate_stride), c);
+      if (a.pre) ring.fetch(stage, kDv, row_of<const T>(a.dv, row, a.channels), c);
     }
     ring.commit();
   };
@@ -343,40 +379,52 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(const NormArgs 
     sw1[i] = sw2[i] = 0.f;
     if (kAll) sb1[i] = sb2[i] = sg[i] = 0.f;
   }
+  // means over a row, the second of a layer norm alone
+  const auto mean_of = [&](float (&p)[2], int kind) {
+    if (kind == FBFFTCONV_NORM_LAYER) {
+      sums(p);
+      p[1] *= per;
+    } else {
+      float one[1] = {p[0]};
+      sums(one);
+      p[0] = one[0], p[1] = 0.f;
+    }
+    p[0] *= per;
+  };
   int stage = 0;
-  for (long long s = worker / splits; s < stretches; s += workers / splits) {
-    const long long end = (s + 1) * stretch;
-    long long row = s * stretch + worker % splits;
+  for (int s = worker / splits; s < stretches; s += workers / splits) {
+    const int end = (s + 1) * stretch;
+    int row = s * stretch + worker % splits;
     if (kRing)
-      for (int k = 0; k < a.stages; ++k) fetch(row + (long long)k * splits, end, stage + k < a.stages ? stage + k : 0);
+      for (int k = 0; k < a.stages; ++k) fetch(row + k * splits, end, shared_gate ? s : row + k * splits, stage + k < a.stages ? stage + k : 0);
     for (; row < end; row += splits, stage = stage + 1 < a.stages ? stage + 1 : 0) {
       const float4 stat = a.stats[row];
       if (kRing) ring.wait();
-      const auto get_u = [&](float (&y)[C]) {
-        if (kRing) ring.template read<T>(stage, kU, c, y);
-        else load_row(static_cast<const T*>(a.u) + row * a.u_stride, c, y);
-      };
-      const auto get_gate = [&](float (&y)[C]) {
-        if (kRing) ring.template read<T>(stage, kGate, c, y);
-        else load_row(static_cast<const T*>(a.gate) + row / a.per_gate * a.gate_stride, c, y);
-      };
-      float x[C], d[C], w[C], y[C];  // x: the block's output, normalised
-      if (need_u) get_u(x);
+      float x[C], d[C], w[C], act[C];  // x: the block's output, normalised
+      if (need_u) {
+        if (kRing) ring.template read<T>(stage, kU, c, x);
+        else load_row(row_of<const T>(a.u, row, a.u_stride), c, x);
+      }
+      if (a.gate_kind) {
+        if (kRing) ring.template read<T>(stage, kGate, c, act);
+        else load_row(row_of<const T>(a.gate, shared_gate ? s : row, a.gate_stride), c, act);
+        activate(act, a.gate_kind);
+      }
       if (a.post) {
 #pragma unroll
         for (int i = 0; i < C; ++i) x[i] = (x[i] - stat.x) * stat.y;
       }
-      // the branch before its gate: what the gate's gradient takes
+      // n: the branch before its gate, which is what the gate's gradient takes; needs w1 in n
       const auto branch = [&](float (&n)[C]) {
         if (a.post) {
-          load_row(a.w1, c, n);
-#pragma unroll
-          for (int i = 0; i < C; ++i) n[i] *= x[i];
           if (a.b1) {
             float b[C];
             load_row(a.b1, c, b);
 #pragma unroll
-            for (int i = 0; i < C; ++i) n[i] += b[i];
+            for (int i = 0; i < C; ++i) n[i] = fmaf(n[i], x[i], b[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < C; ++i) n[i] *= x[i];
           }
         } else {
 #pragma unroll
@@ -385,87 +433,94 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(const NormArgs 
       };
       if (a.dr_out) {
         if (kRing) ring.template read<TR>(stage, kDr, c, d);
-        else load_row(static_cast<const TR*>(a.dr_out) + row * a.channels, c, d);
+        else load_row(row_of<const TR>(a.dr_out, row, a.channels), c, d);
       } else {
 #pragma unroll
         for (int i = 0; i < C; ++i) d[i] = 0.f;
       }
       if (a.pre) {
-        float r[C];
+        float r[C], y[C];
         if (kRing) ring.template read<TR>(stage, kR, c, r);
-        else load_row(static_cast<const TR*>(a.r) + row * a.r_stride, c, r);
+        else load_row(row_of<const TR>(a.r, row, a.r_stride), c, r);
         if (a.u) {
+          if (a.post) load_row(a.w1, c, w);
           branch(w);
           if (a.gate_kind) {
-            get_gate(y);
 #pragma unroll
-            for (int i = 0; i < C; ++i) w[i] *= a.gate_kind == FBFFTCONV_GATE_SIGMOID ? sigmoid(y[i]) : y[i];
+            for (int i = 0; i < C; ++i) w[i] *= act[i];
           }
 #pragma unroll
           for (int i = 0; i < C; ++i) r[i] = fmaf(a.beta, w[i], a.alpha * r[i]);
         }
-        if (kRing) ring.template read<T>(stage, kDv, c, y);
-        else load_row(static_cast<const T*>(a.dv) + row * a.channels, c, y);
         load_row(a.w2, c, w);
-        float p = 0.f, q = 0.f;
+        if (kRing) ring.template read<T>(stage, kDv, c, y);
+        else load_row(row_of<const T>(a.dv, row, a.channels), c, y);
+        float p[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < C; ++i) {
           r[i] = (r[i] - stat.z) * stat.w;
           sw2[i] = fmaf(y[i], r[i], sw2[i]);
           if (kAll) sb2[i] += y[i];
           y[i] *= w[i];  // zero where there is no column
-          p = fmaf(y[i], r[i], p);
-          q += y[i];
+          p[0] = fmaf(y[i], r[i], p[0]);
+          p[1] += y[i];
         }
-        const float2 m = sums(p, q);
-        const float mx = m.x * per, m0 = a.pre == FBFFTCONV_NORM_LAYER ? m.y * per : 0.f;
+        if (kRing) fetch(row + a.stages * splits, end, shared_gate ? s : row + a.stages * splits, stage);
+        if (a.post) load_row(a.w1, c, w);  // on its way during the sums
+        mean_of(p, a.pre);
 #pragma unroll
-        for (int i = 0; i < C; ++i) d[i] = fmaf(stat.w, y[i] - fmaf(r[i], mx, m0), d[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < C; ++i) w[i] = a.alpha * d[i];
-      store_row(static_cast<TR*>(a.dr) + row * a.channels, c, w);
-      if (a.u) {
-#pragma unroll
-        for (int i = 0; i < C; ++i) d[i] *= a.beta;
-        if (a.gate_kind) {
-          branch(w);
-          get_gate(y);
-#pragma unroll
-          for (int i = 0; i < C; ++i) {
-            const float act = a.gate_kind == FBFFTCONV_GATE_SIGMOID ? sigmoid(y[i]) : y[i];
-            const float slope = a.gate_kind == FBFFTCONV_GATE_SIGMOID ? act * (1.f - act) : 1.f;
-            w[i] *= d[i] * slope;
-            d[i] *= act;
-            if (kAll) sg[i] += w[i];
-          }
-          if (!shared_gate) store_row(static_cast<T*>(a.dgate) + row * a.channels, c, w);
-        }
-      }
-      if (kRing) fetch(row + (long long)a.stages * splits, end, stage);
-      if (!a.u) continue;
-      if (a.post) {
+        for (int i = 0; i < C; ++i) d[i] = fmaf(stat.w, y[i] - fmaf(r[i], p[0], p[1]), d[i]);
+      } else {
+        if (kRing) fetch(row + a.stages * splits, end, shared_gate ? s : row + a.stages * splits, stage);
         load_row(a.w1, c, w);
-        float p = 0.f, q = 0.f;
+      }
+      {
+        float out[C];
+#pragma unroll
+        for (int i = 0; i < C; ++i) out[i] = a.alpha * d[i];
+        store_row(row_of<TR>(a.dr, row, a.channels), c, out);
+      }
+      if (!a.u) continue;
+#pragma unroll
+      for (int i = 0; i < C; ++i) d[i] *= a.beta;
+      if (a.gate_kind) {
+        float n[C];
+#pragma unroll
+        for (int i = 0; i < C; ++i) n[i] = w[i];
+        branch(n);
+#pragma unroll
+        for (int i = 0; i < C; ++i) n[i] *= d[i];
+        if (a.gate_kind == FBFFTCONV_GATE_SIGMOID) {
+#pragma unroll
+          for (int i = 0; i < C; ++i) n[i] *= fmaf(-act[i], act[i], act[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          d[i] *= act[i];
+          if (kAll) sg[i] += n[i];
+        }
+        if (!shared_gate) store_row(row_of<T>(a.dgate, row, a.channels), c, n);
+      }
+      if (a.post) {
+        float p[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < C; ++i) {
           sw1[i] = fmaf(d[i], x[i], sw1[i]);
           if (kAll) sb1[i] += d[i];
           d[i] *= w[i];
-          p = fmaf(d[i], x[i], p);
-          q += d[i];
+          p[0] = fmaf(d[i], x[i], p[0]);
+          p[1] += d[i];
         }
-        const float2 m = sums(p, q);
-        const float mx = m.x * per, m0 = a.post == FBFFTCONV_NORM_LAYER ? m.y * per : 0.f;
+        mean_of(p, a.post);
 #pragma unroll
-        for (int i = 0; i < C; ++i) d[i] = stat.y * (d[i] - fmaf(x[i], mx, m0));
+        for (int i = 0; i < C; ++i) d[i] = stat.y * (d[i] - fmaf(x[i], p[0], p[1]));
       }
-      store_row(static_cast<T*>(a.du) + row * a.channels, c, d);
+      store_row(row_of<T>(a.du, row, a.channels), c, d);
     }
     if constexpr (kAll) {
       if (shared_gate) {
         if (a.gate_sums) store_row(a.gate_sums + (long long)worker * a.channels, c, sg);
-        else store_row(static_cast<T*>(a.dgate) + s * a.channels, c, sg);
+        else store_row(row_of<T>(a.dgate, s, a.channels), c, sg);
 #pragma unroll
         for (int i = 0; i < C; ++i) sg[i] = 0.f;
       }
@@ -544,13 +599,15 @@ Shape forward_shape(int channels, bool vectors) {
 }
 // `all`: sums of biases' and shared gates' gradients are held too, which leaves registers for fewer columns.
 Shape backward_shape(int channels, bool vectors, bool all) {
-  if (vectors && channels <= 8192) return shape_of(channels, channels > (all ? 4096 : 2048) ? 16 : 8, true);
+  if (vectors && channels <= 8192) return shape_of(channels, channels > 4096 ? 16 : 8, true);
   return shape_of(channels, channels > 4096 ? 16 : 8, false);
 }
 
 int check_desc(const fbfftconv_norm_desc* d) {
   if (!d) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "null argument");
   if (d->rows < 0 || d->channels <= 0) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "rows and channels must be positive");
+  if (d->rows > kMostRows || d->u_stride > kMostStride || d->r_stride > kMostStride || d->gate_stride > kMostStride)
+    return op_fail(FBFFTCONV_ERR_UNSUPPORTED_SIZE, "more than 2^30 rows, or elements between rows");
   if (d->channels > kMostChannels) return op_fail(FBFFTCONV_ERR_UNSUPPORTED_SIZE, "more than %d channels", kMostChannels);
   if (!known_type(d->type) || !known_type(d->residual_type) ||
       (d->residual_type != d->type && d->residual_type != FBFFTCONV_FLOAT32))
@@ -568,12 +625,12 @@ int check_desc(const fbfftconv_norm_desc* d) {
 
 NormArgs common_args(const fbfftconv_norm_desc& d) {
   NormArgs a{};
-  a.rows = d.rows, a.channels = d.channels;
+  a.rows = (int)d.rows, a.channels = d.channels;
   a.post = d.post, a.pre = d.pre, a.gate_kind = d.gate;
-  a.u_stride = d.u_stride ? d.u_stride : d.channels;
-  a.r_stride = d.r_stride ? d.r_stride : d.channels;
-  a.gate_stride = d.gate_stride ? d.gate_stride : d.channels;
-  a.per_gate = d.gate && d.gate_rows ? d.rows / d.gate_rows : 1;
+  a.u_stride = d.u_stride ? (int)d.u_stride : d.channels;
+  a.r_stride = d.r_stride ? (int)d.r_stride : d.channels;
+  a.gate_stride = d.gate_stride ? (int)d.gate_stride : d.channels;
+  a.per_gate = d.gate && d.gate_rows ? (int)(d.rows / d.gate_rows) : 1;
   a.eps = d.eps, a.alpha = d.residual_scale, a.beta = d.branch_scale;
   return a;
 }
@@ -623,8 +680,9 @@ cudaError_t forward(const NormArgs& a, const Shape& s, cudaStream_t stream) {
     return s.columns == 8 ? launch_rows(norm_forward_kernel<T, TR, 8, 1024, false>, a, s, grid, 0, stream)
                           : launch_rows(norm_forward_kernel<T, TR, 16, 1024, false>, a, s, grid, 0, stream);
   const size_t stage = (size_t)s.threads * s.columns * (2 * sizeof(T) + sizeof(TR));
-  return s.columns == 8 ? launch_rows(norm_forward_kernel<T, TR, 8, 256, true>, a, s, grid, stage, stream)
-                        : launch_rows(norm_forward_kernel<T, TR, 16, 512, true>, a, s, grid, stage, stream);
+  if (s.columns == 8) return launch_rows(norm_forward_kernel<T, TR, 8, 256, true>, a, s, grid, stage, stream);
+  return s.threads <= 320 ? launch_rows(norm_forward_kernel<T, TR, 16, 320, true>, a, s, grid, stage, stream)
+                          : launch_rows(norm_forward_kernel<T, TR, 16, 512, true>, a, s, grid, stage, stream);
 }
 
 template <typename T, typename TR, bool kAll>

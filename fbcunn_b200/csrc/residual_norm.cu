@@ -104,12 +104,18 @@ __device__ __forceinline__ void store_vector(T* p, const float* x) {
   }
 }
 
-// x = the row's columns as fp32, zero where there is none.
+// x = the row's columns as fp32.  Where there is none: zero; in the ring's kernels, whose threads have whole vectors or
+// none, any other of the row's, which keeps the loads free of branches (sum_of leaves it out).
 template <typename T, int C, int kVec, bool kRing>
 __device__ __forceinline__ void load_row(const T* row, const Columns<C, kVec, kRing>& c, float (&x)[C]) {
+  if constexpr (kRing) {
+#pragma unroll
+    for (int i = 0; i < C; i += kVec) load_vector<T, kVec>(row + (c.has(i) ? c.at(i) : 0), x + i);
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < C; ++i) x[i] = 0.f;
-  if (kRing || c.vectors) {
+  if (c.vectors) {
 #pragma unroll
     for (int i = 0; i < C; i += kVec)
       if (c.has(i)) load_vector<T, kVec>(row + c.at(i), x + i);
@@ -175,12 +181,23 @@ struct Ring {
           x[i + 2 * k] = f.x, x[i + 2 * k + 1] = f.y;
         }
       }
-      if (!c.has(i))
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) x[i + k] = 0.f;  // what lies there was never written
     }
   }
 };
+
+// The sum of a thread's columns of a row: what lies in vectors that are not the row's stays out, whatever it holds.
+template <int C, int kVec, bool kRing, typename F>
+__device__ __forceinline__ float sum_of(const Columns<C, kVec, kRing>& c, F term) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < C; i += kVec) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = i; k < i + kVec; ++k) t = term(k, t);
+    s += !kRing || c.has(i) ? t : 0.f;
+  }
+  return s;
+}
 
 // Sums over the lanes of a row, for everyone: shuffles within a warp, then every thread adds the warps' sums in their
 // order.  Two exchanges in turn use the two halves of `part`: a warp that is through with one cannot reach the next but
@@ -226,19 +243,13 @@ __device__ __forceinline__ float2 normalise(float (&x)[C], int kind, const Colum
   const float per = 1.f / (float)c.channels;
   float mean = 0.f;
   if (kind == FBFFTCONV_NORM_LAYER) {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < C; ++i) s += x[i];
-    float one[1] = {s};
+    float one[1] = {sum_of(c, [&](int i, float t) { return t + x[i]; })};
     sums(one);
     mean = one[0] * per;
 #pragma unroll
-    for (int i = 0; i < C; ++i) x[i] = c.has(i) ? x[i] - mean : 0.f;
+    for (int i = 0; i < C; ++i) x[i] = kRing || c.has(i) ? x[i] - mean : 0.f;
   }
-  float q = 0.f;
-#pragma unroll
-  for (int i = 0; i < C; ++i) q = fmaf(x[i], x[i], q);
-  float one[1] = {q};
+  float one[1] = {sum_of(c, [&](int i, float t) { return fmaf(x[i], x[i], t); })};
   sums(one);
   return make_float2(mean, 1.f / sqrtf(fmaf(one[0], per, eps)));
 }
@@ -455,16 +466,15 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(const NormArgs 
         load_row(a.w2, c, w);
         if (kRing) ring.template read<T>(stage, kDv, c, y);
         else load_row(row_of<const T>(a.dv, row, a.channels), c, y);
-        float p[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < C; ++i) {
           r[i] = (r[i] - stat.z) * stat.w;
           sw2[i] = fmaf(y[i], r[i], sw2[i]);
           if (kAll) sb2[i] += y[i];
-          y[i] *= w[i];  // zero where there is no column
-          p[0] = fmaf(y[i], r[i], p[0]);
-          p[1] += y[i];
+          y[i] *= w[i];
         }
+        float p[2] = {sum_of(c, [&](int i, float t) { return fmaf(y[i], r[i], t); }), 0.f};
+        if (a.pre == FBFFTCONV_NORM_LAYER) p[1] = sum_of(c, [&](int i, float t) { return t + y[i]; });
         if (kRing) fetch(row + a.stages * splits, end, shared_gate ? s : row + a.stages * splits, stage);
         if (a.post) load_row(a.w1, c, w);  // on its way during the sums
         mean_of(p, a.pre);
@@ -502,15 +512,14 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(const NormArgs 
         if (!shared_gate) store_row(row_of<T>(a.dgate, row, a.channels), c, n);
       }
       if (a.post) {
-        float p[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < C; ++i) {
           sw1[i] = fmaf(d[i], x[i], sw1[i]);
           if (kAll) sb1[i] += d[i];
           d[i] *= w[i];
-          p[0] = fmaf(d[i], x[i], p[0]);
-          p[1] += d[i];
         }
+        float p[2] = {sum_of(c, [&](int i, float t) { return fmaf(d[i], x[i], t); }), 0.f};
+        if (a.post == FBFFTCONV_NORM_LAYER) p[1] = sum_of(c, [&](int i, float t) { return t + d[i]; });
         mean_of(p, a.post);
 #pragma unroll
         for (int i = 0; i < C; ++i) d[i] = stat.y * (d[i] - fmaf(x[i], p[0], p[1]));

@@ -162,6 +162,8 @@ _SIGNATURES = {
     "fbfftconv_recurrence_workspace_bytes": (c_size_t, [c_void_p]),
     "fbfftconv_recurrence": (c_int, [c_void_p] * 10),
     "fbfftconv_recurrence_backward": (c_int, [c_void_p] * 14 + [c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "fbfftconv_recurrence_status": (c_int, [c_int]),
+    "fbfftconv_recurrence_wait_selftest": (c_int, [c_void_p]),
     "fbfftconv_recurrence_step": (c_int, [c_void_p] * 8),
     "fbfftconv_profile_enable": (c_int, [c_void_p, c_int]),
     "fbfftconv_profile_reset": (c_int, [c_void_p]),

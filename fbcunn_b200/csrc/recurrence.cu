@@ -58,16 +58,28 @@ struct RecArgs {
   int channels, wide_offsets, cluster;
 };
 
-__device__ __forceinline__ long long offset_at(const RecArgs& a, long long i) {
+// Offsets of up to this many sequences are kept in shared memory: a search is a chain of loads.
+constexpr int kKeptOffsets = 512;
+
+__device__ __forceinline__ long long load_offset(const RecArgs& a, long long i) {
   const long long v = a.wide_offsets ? static_cast<const long long*>(a.offsets)[i] : static_cast<const int*>(a.offsets)[i];
   return v < 0 ? 0 : v > a.rows ? a.rows : v;  // a bad offset must not lead out of the tensors
+}
+
+__device__ __forceinline__ long long offset_at(const RecArgs& a, const long long* kept, long long i) {
+  return a.sequences <= kKeptOffsets ? kept[i] : load_offset(a, i);
+}
+__device__ __forceinline__ void keep_offsets(const RecArgs& a, long long* kept) {
+  if (a.offsets && a.sequences <= kKeptOffsets)
+    for (int i = threadIdx.x; i <= a.sequences; i += kThreads) kept[i] = load_offset(a, i);
+  __syncthreads();
 }
 
 // The sequence that a row belongs to, and the rows where it begins and ends.
 struct Sequence {
   long long index, begin, end;
 };
-__device__ __forceinline__ Sequence sequence_of(const RecArgs& a, long long row) {
+__device__ __forceinline__ Sequence sequence_of(const RecArgs& a, const long long* kept, long long row) {
   if (!a.offsets) {
     const long long i = (a.rows | a.length) >> 32 ? row / a.length : (uint32_t)row / (uint32_t)a.length;
     return {i, i * a.length, (i + 1) * a.length};
@@ -75,24 +87,24 @@ __device__ __forceinline__ Sequence sequence_of(const RecArgs& a, long long row)
   long long lo = 0, hi = a.sequences;  // the last one that begins at or before the row
   while (hi - lo > 1) {
     const long long mid = (lo + hi) >> 1;
-    if (offset_at(a, mid) <= row) lo = mid;
+    if (offset_at(a, kept, mid) <= row) lo = mid;
     else hi = mid;
   }
-  return {lo, offset_at(a, lo), offset_at(a, lo + 1)};
+  return {lo, offset_at(a, kept, lo), offset_at(a, kept, lo + 1)};
 }
 
 // The sequence that a row belongs to, for the few rows that begin or end one: kept out of the loops' code.
-__device__ __noinline__ long long index_of(const RecArgs& a, long long row) { return sequence_of(a, row).index; }
+__device__ __noinline__ long long index_of(const RecArgs& a, const long long* kept, long long row) { return sequence_of(a, kept, row).index; }
 
 // Which of a warp's rows begin a sequence, and which end one.  `in`, the sequence that its rows were in last, is looked
 // up anew only where they have left it; most rounds lie within one sequence.
 struct Borders {
   uint32_t first, last;
 };
-__device__ __forceinline__ Borders borders(const RecArgs& a, long long row, int n, Sequence& in) {
+__device__ __forceinline__ Borders borders(const RecArgs& a, const long long* kept, long long row, int n, Sequence& in) {
   Borders b{0, 0};
   if (n <= 0) return b;
-  if (row < in.begin || row >= in.end) in = sequence_of(a, row);
+  if (row < in.begin || row >= in.end) in = sequence_of(a, kept, row);
   if (row > in.begin && in.end - row > n) return b;
   if (row == in.begin) b.first = 1;
   while (in.end > row && in.end - row <= n) {
@@ -100,7 +112,7 @@ __device__ __forceinline__ Borders borders(const RecArgs& a, long long row, int 
     b.last |= 1u << (k - 1);
     if (k == n) break;
     b.first |= 1u << k;
-    const Sequence next = sequence_of(a, in.end);
+    const Sequence next = sequence_of(a, kept, in.end);
     if (next.end <= in.end) break;  // offsets that do not rise
     in = next;
   }
@@ -290,39 +302,102 @@ template <int V>
 struct Exchange {
   Stretch<V> part[kWarps][32];
   Stretch<V> whole[2][kMostCluster][32];
+  uint64_t arrived[2];  // mbarriers: the cluster's stretches of a round are there
+  int gave_up;
 };
 
-// `mine`: this warp's stretch; returns the value that enters it and moves `carry` behind the whole round.
+__device__ int wait_error;  // set when a wait for a cluster's stretches ran out
+
+constexpr uint32_t kMostPolls = 1u << 20;  // of a microsecond: about a second, where a round takes some microseconds
+
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ bool wait_phase(uint32_t barrier, uint32_t parity, uint32_t polls) {
+  for (uint32_t i = 0; i < polls; ++i) {
+    uint32_t done;
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(done) : "r"(barrier), "r"(parity), "r"(1000u) : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+
 template <int V>
-__device__ __forceinline__ Vec<V> exchange(Exchange<V>& x, int half, int order, int rank, int blocks, const Stretch<V>& mine,
-                                           Vec<V>& carry) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void start_exchange(Exchange<V>& x, int blocks) {
+  if (blocks == 1) return;
+  if (threadIdx.x == 0) {
+    x.gave_up = 0;
+    for (int h = 0; h < 2; ++h) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&x.arrived[h])) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  cg::this_cluster().sync();
+}
+
+// Writes a stretch into another block's shared memory and counts its bytes there.
+__device__ __forceinline__ void send(uint32_t to, uint32_t barrier, int block, const Stretch<2>& s) {
+  asm volatile(
+      "{ .reg .b32 a, b; mapa.shared::cluster.u32 a, %0, %2; mapa.shared::cluster.u32 b, %1, %2;\n"
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [a], {%3, %4, %5, %6}, [b]; }"
+      ::"r"(to), "r"(barrier), "r"(block), "f"(s.A.x), "f"(s.A.y), "f"(s.H.x), "f"(s.H.y) : "memory");
+}
+__device__ __forceinline__ void send(uint32_t to, uint32_t barrier, int block, const Stretch<1>& s) {
+  asm volatile(
+      "{ .reg .b32 a, b; mapa.shared::cluster.u32 a, %0, %2; mapa.shared::cluster.u32 b, %1, %2;\n"
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [a], {%3, %4}, [b]; }"
+      ::"r"(to), "r"(barrier), "r"(block), "f"(s.A.x), "f"(s.H.x) : "memory");
+}
+
+// `mine`: this warp's stretch; returns the value that enters it and moves `carry` behind the whole round.  A block's
+// stretch goes to all blocks of the cluster with the bytes counted on their mbarriers: a cluster's barrier would have
+// waited for the outputs that are on their way to memory too.  A block sends a round's stretch after all of its warps
+// have read the round's before, so that nothing arrives in a buffer that is still read, and it has all that is sent to it
+// when it leaves.
+template <int V>
+__device__ __forceinline__ Vec<V> exchange(Exchange<V>& x, uint32_t round, int order, int rank, int blocks,
+                                           const Stretch<V>& mine, Vec<V>& carry) {
+  const int lane = threadIdx.x & 31, half = round & 1;
   Stretch<V>(*const part)[32] = blocks == 1 && half ? x.whole[0] : x.part;
   part[order][lane] = mine;
   __syncthreads();
   Stretch<V> before = nothing<V>();
+#pragma unroll 4
   for (int w = 0; w < order; ++w) before = join(before, part[w][lane]);
   Stretch<V> all = join(before, mine);
+#pragma unroll 4
   for (int w = order + 1; w < kWarps; ++w) all = join(all, part[w][lane]);
   if (blocks == 1) {
     const Vec<V> enter = apply(before, carry);
     carry = apply(all, carry);
     return enter;
   }
-  cg::cluster_group cluster = cg::this_cluster();
-  for (int k = order; k < blocks; k += kWarps) cluster.map_shared_rank(&x, k)->whole[half][rank][lane] = all;
-  cluster.sync();
+  const uint32_t barrier = shared_address(&x.arrived[half]);
+  if (threadIdx.x == 0)
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"((uint32_t)(blocks * 32 * sizeof(Stretch<V>))) : "memory");
+  for (int k = order; k < blocks; k += kWarps) send(shared_address(&x.whole[half][rank][lane]), barrier, k, all);
+  if (!*reinterpret_cast<volatile int*>(&x.gave_up) && !wait_phase(barrier, round >> 1 & 1, kMostPolls)) {
+    x.gave_up = 1;  // the other waits of this block then run out at once: its results are lost, the kernel ends
+    wait_error = 1;
+  }
+#pragma unroll 4
   for (int k = 0; k < rank; ++k) carry = apply(x.whole[half][k][lane], carry);
   const Vec<V> enter = apply(before, carry);
+#pragma unroll 4
   for (int k = rank; k < blocks; ++k) carry = apply(x.whole[half][k][lane], carry);
   return enter;
 }
 
+// Starts a wait that nothing ends, with a limit of a few polls: 1 when it gave up.
+__global__ void wait_probe_kernel(int* gave_up) {
+  __shared__ uint64_t barrier;
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&barrier)) : "memory");
+  *gave_up = !wait_phase(shared_address(&barrier), 0, 4);
+}
+
 // The rows of this block's segment: [begin, end).
-__device__ __forceinline__ void segment_rows(const RecArgs& a, long long& begin, long long& end) {
+__device__ __forceinline__ void segment_rows(const RecArgs& a, const long long* kept, long long& begin, long long& end) {
   if (a.offsets) {
-    begin = offset_at(a, 0);
-    end = offset_at(a, a.sequences);
+    begin = offset_at(a, kept, 0);
+    end = offset_at(a, kept, a.sequences);
   } else {
     const long long first = (long long)blockIdx.y * a.per_segment;
     const long long last = min(first + a.per_segment, a.sequences);
@@ -332,10 +407,10 @@ __device__ __forceinline__ void segment_rows(const RecArgs& a, long long& begin,
 
 // Sequences without rows hand their state on.
 template <int V>
-__device__ __forceinline__ void pass_empty(const RecArgs& a, const float* from, float* to, int channel, bool on) {
+__device__ __forceinline__ void pass_empty(const RecArgs& a, const long long* kept, const float* from, float* to, int channel, bool on) {
   if (!to || blockIdx.y || (!a.offsets && a.length > 0)) return;
   for (long long s = threadIdx.x >> 5; s < a.sequences; s += kWarps) {
-    if (a.offsets && offset_at(a, s + 1) > offset_at(a, s)) continue;
+    if (a.offsets && offset_at(a, kept, s + 1) > offset_at(a, kept, s)) continue;
 #pragma unroll
     for (int v = 0; v < V; ++v)
       if (on) to[s * a.channels + channel + v] = from ? from[s * a.channels + channel + v] : 0.f;
@@ -346,16 +421,18 @@ template <typename T, int V, bool kGate>
 __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const __grid_constant__ RecArgs a) {
   constexpr int L = kForwardRows, kTile = kWarps * L;
   extern __shared__ __align__(16) char staged[];
-  __shared__ Exchange<V> shared;
+  __shared__ __align__(16) Exchange<V> shared;
+  __shared__ long long kept[kKeptOffsets + 1];
   grid_dependency_wait();
+  keep_offsets(a, kept);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int blocks = a.cluster, rank = blockIdx.x % blocks;
   const int channel = (blockIdx.x / blocks * 32 + lane) * V;
   const bool on = channel < a.channels;
   const int c = on ? channel : 0;
   long long begin, end;
-  segment_rows(a, begin, end);
-  if (rank == 0) pass_empty<V>(a, a.state0, a.state, c, on);
+  segment_rows(a, kept, begin, end);
+  if (rank == 0) pass_empty<V>(a, kept, a.state0, a.state, c, on);
   const long long tiles = (end - begin + kTile - 1) / kTile, rounds = (tiles + blocks - 1) / blocks;
   const Words<T, V, L> words{staged + 4 * threadIdx.x};
   enum { kX, kG, kZ };  // slots
@@ -364,6 +441,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const _
   const T* const z0 = static_cast<const T*>(a.z) + c;
   const Vec<V> bias = a.bias ? load_floats<V>(a.bias + c) : all_of<V>(0.f);
   Vec<V> carry = all_of<V>(0.f);
+  start_exchange(shared, blocks);
   const auto row_of = [&](long long round) { return begin + ((round * blocks + rank) * kWarps + warp) * L; };
   const auto rows_at = [&](long long row) { return (int)max(0ll, min((long long)L, end - row)); };
   const auto fetch_inputs = [&](long long round) {
@@ -388,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const _
     const T* const gs = g0 + row * a.g_stride;
     const T* const zs = z0 + row * a.z_stride;
     words.wait();
-    const Borders at = borders(a, row, n, in);
+    const Borders at = borders(a, kept, row, n, in);
     const bool within = n == L && at.first == 0 && at.last == 0;  // all rows there, none at a sequence's border
     Vec<V> A[L], B[L];
     Stretch<V> mine = nothing<V>();
@@ -399,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const _
           gate_of(words.read(kG, gs, a.g_stride, i) + bias, A[i], B[i]);
           B[i] = B[i] * words.read(kX, xs, a.x_stride, i);
           if (!plain && (at.first >> i & 1)) {  // the row takes the initial state, whatever comes before it
-            if (a.state0) B[i] = fma(A[i], load_floats<V>(a.state0 + index_of(a, row + i) * a.channels + c), B[i]);
+            if (a.state0) B[i] = fma(A[i], load_floats<V>(a.state0 + index_of(a, kept, row + i) * a.channels + c), B[i]);
             mine = Stretch<V>{all_of<V>(-1.f), B[i]};
           } else {
             const bool cut = !plain && mine.A.x < 0.f;
@@ -413,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const _
     if (within) scan(std::true_type{});
     else scan(std::false_type{});
     fetch_inputs(round + 1);
-    Vec<V> h = exchange(shared, (int)(round & 1), warp, rank, blocks, mine, carry);
+    Vec<V> h = exchange(shared, (uint32_t)round, warp, rank, blocks, mine, carry);
     words.wait();
     if (a.checkpoints && n > 0 && on && (row - begin) % kCheckpoint == 0)
       store_floats(a.checkpoints + (blockIdx.y * a.checkpoints_per_segment + (row - begin) / kCheckpoint) * a.channels + c, h);
@@ -431,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const _
         }
         if (on) store_word<T, V>(y + i * a.y_stride, out);
         if (!plain && (at.last >> i & 1) && a.state && on)
-          store_floats(a.state + index_of(a, row + i) * a.channels + c, h);
+          store_floats(a.state + index_of(a, kept, row + i) * a.channels + c, h);
       }
     };
     if (within) emit(std::true_type{});
@@ -444,17 +522,19 @@ template <typename T, int V, bool kGate>
 __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const __grid_constant__ RecArgs a) {
   constexpr int L = kBackwardRows, kTile = kWarps * L;
   extern __shared__ __align__(16) char staged[];
-  __shared__ Exchange<V> shared;
+  __shared__ __align__(16) Exchange<V> shared;
   __shared__ Stretch<V> states[2][kWarps][32];
+  __shared__ long long kept[kKeptOffsets + 1];
   grid_dependency_wait();
+  keep_offsets(a, kept);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int blocks = a.cluster, rank = blockIdx.x % blocks;
   const int channel = (blockIdx.x / blocks * 32 + lane) * V;
   const bool on = channel < a.channels;
   const int c = on ? channel : 0;
   long long begin, end;
-  segment_rows(a, begin, end);
-  if (rank == 0) pass_empty<V>(a, a.dstate, a.dstate0, c, on);
+  segment_rows(a, kept, begin, end);
+  if (rank == 0) pass_empty<V>(a, kept, a.dstate, a.dstate0, c, on);
   const long long tiles = (end - begin + kTile - 1) / kTile, rounds = (tiles + blocks - 1) / blocks;
   const Words<T, V, L> words{staged + 4 * threadIdx.x};
   enum { kX, kG = 2, kDy, kZ };  // slots: x has two, it is read to the end of its round
@@ -464,6 +544,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
   const T* const z0 = static_cast<const T*>(a.z) + c;
   const Vec<V> bias = a.bias ? load_floats<V>(a.bias + c) : all_of<V>(0.f);
   Vec<V> carry = all_of<V>(0.f), dbias = all_of<V>(0.f);
+  start_exchange(shared, blocks);
   // the last rows come first
   const auto tile_of = [&](long long round) { return tiles - 1 - (round * blocks + rank); };
   const auto row_of = [&](long long round) { return begin + (tile_of(round) * kWarps + warp) * L; };
@@ -497,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
     Vec<V> h = tile < 0 ? all_of<V>(0.f)
                         : load_floats<V>(a.checkpoints + (blockIdx.y * a.checkpoints_per_segment + tile) * a.channels + c);
     words.wait();
-    const Borders at = borders(a, row, n, in);
+    const Borders at = borders(a, kept, row, n, in);
     const bool within = n == L && at.first == 0 && at.last == 0;  // all rows there, none at a sequence's border
     // the states of the warp's rows: its stretch, those of the warps before it, and from row to row
     Vec<V> A[L], B[L], P[L], E[L];  // gates, states before each row, what enters each row from its output
@@ -509,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
           gate_of(words.read(kG, gs, a.g_stride, i) + bias, A[i], B[i]);
           const Vec<V> in_x = B[i] * words.read(kX + stage, xs, a.x_stride, i);
           if (!plain && (at.first >> i & 1)) {
-            P[i] = a.state0 ? load_floats<V>(a.state0 + index_of(a, row + i) * a.channels + c) : all_of<V>(0.f);
+            P[i] = a.state0 ? load_floats<V>(a.state0 + index_of(a, kept, row + i) * a.channels + c) : all_of<V>(0.f);
             mine = Stretch<V>{all_of<V>(-1.f), fma(A[i], P[i], in_x)};
           } else {
             const bool cut = !plain && mine.A.x < 0.f;
@@ -549,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
           if (a.dz && on) store_word<T, V>(dz + i * a.dz_stride, (ds * h) * slope);
         }
         if (!plain && (at.last >> i & 1) && a.dstate)
-          E[i] = E[i] + load_floats<V>(a.dstate + index_of(a, row + i) * a.channels + c);
+          E[i] = E[i] + load_floats<V>(a.dstate + index_of(a, kept, row + i) * a.channels + c);
       }
 #pragma unroll
       for (int i = L - 1; i >= 0; --i) {
@@ -562,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
     if (within) through(std::true_type{});
     else through(std::false_type{});
     fetch_outputs(round + 1);
-    Vec<V> d = exchange(shared, stage, kWarps - 1 - warp, rank, blocks, mine, carry);
+    Vec<V> d = exchange(shared, (uint32_t)round, kWarps - 1 - warp, rank, blocks, mine, carry);
     T* dx = static_cast<T*>(a.dx) + row * a.dx_stride + c;
     T* dg = static_cast<T*>(a.dg) + row * a.dg_stride + c;
     const auto emit = [&](auto plain) {
@@ -578,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
         if (a.dx && on) store_word<T, V>(dx + i * a.dx_stride, out);
         if (a.dg && on) store_word<T, V>(dg + i * a.dg_stride, gate);
         if (!plain && (at.first >> i & 1)) {
-          if (a.dstate0 && on) store_floats(a.dstate0 + index_of(a, row + i) * a.channels + c, d);
+          if (a.dstate0 && on) store_floats(a.dstate0 + index_of(a, kept, row + i) * a.channels + c, d);
           d = all_of<V>(0.f);
         }
       }
@@ -904,6 +985,33 @@ int fbfftconv_recurrence_backward(const fbfftconv_recurrence_desc* desc, const v
   const cudaError_t e = launch_dependent(recurrence_sum_kernel, dim3((d.channels + 127) / 128), 128, 0, cuda_stream,
                                          static_cast<const float*>(workspace), grad_bias, parts, d.channels, scale, accumulate);
   return e == cudaSuccess ? FBFFTCONV_OK : op_cuda_fail(e, "recurrence, sums");
+}
+
+int fbfftconv_recurrence_status(int reset) {
+  int code = 0;
+  const int zero = 0;
+  if (cudaMemcpyFromSymbol(&code, wait_error, sizeof(code)) != cudaSuccess ||
+      (reset && code && cudaMemcpyToSymbol(wait_error, &zero, sizeof(zero)) != cudaSuccess)) {
+    cudaGetLastError();
+    return -1;
+  }
+  return code;
+}
+
+int fbfftconv_recurrence_wait_selftest(fbfftconv_stream stream) {
+  int* out = nullptr;
+  cudaError_t e = cudaMalloc(&out, sizeof(int));
+  int gave_up = 0;
+  if (e == cudaSuccess) {
+    count_launch();
+    wait_probe_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(out);
+    e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
+    if (e == cudaSuccess) e = cudaMemcpy(&gave_up, out, sizeof(int), cudaMemcpyDeviceToHost);
+    cudaFree(out);
+  }
+  if (e != cudaSuccess) return op_cuda_fail(e, "recurrence, wait");
+  return gave_up ? FBFFTCONV_OK : op_fail(FBFFTCONV_ERR_CUDA, "the wait did not give up");
 }
 
 int fbfftconv_recurrence_step(const fbfftconv_recurrence_desc* desc, const void* x, const void* g, const void* z,

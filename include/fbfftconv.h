@@ -396,6 +396,12 @@ int fbfftconv_recurrence_backward(const fbfftconv_recurrence_desc* desc, const v
 int fbfftconv_recurrence_step(const fbfftconv_recurrence_desc* desc, const void* x, const void* g, const void* z,
                               const float* bias, float* state, void* y, fbfftconv_stream stream);
 
+/* Long sequences of few channels go over clusters of blocks that wait for one another's results; the waits are bounded.
+ * 0, or 1 when one has run out since the last reset: that call's results are lost.  -1: the query failed.  Waits for
+ * the device.  The self-test makes such a wait run out: FBFFTCONV_OK when it gave up as designed. */
+int fbfftconv_recurrence_status(int reset);
+int fbfftconv_recurrence_wait_selftest(fbfftconv_stream stream);
+
 /* ---- norms before and after a residual block ------------------------------------------------
  * One call at the border between two blocks of a residual network: the norm after the block that ends, its gate, the
  * residual sum with its scales, and the norm before the block that begins.

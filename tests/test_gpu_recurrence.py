@@ -366,3 +366,12 @@ def test_refusals():
     assert lib.fbfftconv_recurrence(m._desc_ref, *p, None, None, host.data_ptr(), state.data_ptr(), None, None) == capi.ERR_INVALID_ARGUMENT
     assert lib.fbfftconv_recurrence(m._desc_ref, *p, None, h0.data_ptr(), m.output.data_ptr(), h0.data_ptr(), None, None) == capi.ERR_INVALID_ARGUMENT
     assert capi.kernel_launches() == launches
+
+
+def test_a_wait_that_nothing_ends_gives_up():
+    """Clusters of blocks wait for one another's results; the limit of such a wait, on a barrier nothing completes."""
+    lib = capi.lib()
+    capi.check(lib.fbfftconv_recurrence_wait_selftest(torch.cuda.current_stream().cuda_stream))
+    m, table, dy, h0, dlast = make((1, 3000), 1, 64, BF, seed=7)
+    check(m, table, dy, h0, dlast)
+    assert lib.fbfftconv_recurrence_status(0) == 0

@@ -64,6 +64,7 @@ struct Common {
   long long* steps;      // steps done; blocks that are through with this launch
   uint32_t seed;
   int tensors, blocks, advance;
+  int run;               // blocks in a row that a warp takes, or 0: every so many-th, as many as there are warps
 };
 
 // 4 KB of parameters reach every device; larger tables take the extended limit.
@@ -365,9 +366,11 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
   }
   __syncthreads();
   const Step s = shared;
-  const int warps = gridDim.x * kWarps;
+  const int warps = gridDim.x * kWarps, warp = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int stride = c.run ? 1 : warps;
+  const int last = c.run ? min(c.blocks, (warp + 1) * c.run) : c.blocks;
   int k = 0;
-  for (int b = blockIdx.x * kWarps + (threadIdx.x >> 5); b < c.blocks;) {
+  for (int b = c.run ? warp * c.run : warp; b < last;) {
     int lo = k, hi = c.tensors;  // the tensor that block b belongs to
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -376,10 +379,10 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     }
     k = lo;
     const Entry& e = t.entry[k];
-    const int end = k + 1 < c.tensors ? t.entry[k + 1].first : c.blocks;
-    if (e.scale1) update_tensor<true>(e, c, s, b - e.first, end - e.first, warps);
-    else update_tensor<false>(e, c, s, b - e.first, end - e.first, warps);
-    b += (end - b + warps - 1) / warps * warps;
+    const int end = min(last, k + 1 < c.tensors ? t.entry[k + 1].first : c.blocks);
+    if (e.scale1) update_tensor<true>(e, c, s, b - e.first, end - e.first, stride);
+    else update_tensor<false>(e, c, s, b - e.first, end - e.first, stride);
+    b += (end - b + stride - 1) / stride * stride;
   }
   if (!c.advance) return;
   // the step's last launch counts it, once every block has read the count
@@ -425,6 +428,7 @@ cudaError_t launch(const fbfftconv_adamw* h, const int* tensors, int count, cons
   const int rounds = 2 * packed_blocks > blocks ? 1 : 16;
   const long long most = (long long)sm_count() * resident * rounds, need = (blocks + kWarps - 1) / kWarps;
   const int grid = (int)(need < 1 ? 1 : need < most ? need : most);
+  if (rounds == 1) table.c.run = (int)((blocks + (long long)grid * kWarps - 1) / ((long long)grid * kWarps));
   count_launch();
   return launch_dependent(adamw_kernel<N>, dim3(grid), kThreads, 0, stream, table);
 }

@@ -111,18 +111,18 @@ __device__ __forceinline__ void load_row(const T* row, const Columns<C, kVec, kR
   if constexpr (kRing) {
 #pragma unroll
     for (int i = 0; i < C; i += kVec) load_vector<T, kVec>(row + (c.has(i) ? c.at(i) : 0), x + i);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < C; ++i) x[i] = 0.f;
-  if (c.vectors) {
-#pragma unroll
-    for (int i = 0; i < C; i += kVec)
-      if (c.has(i)) load_vector<T, kVec>(row + c.at(i), x + i);
   } else {
 #pragma unroll
-    for (int i = 0; i < C; ++i)
-      if (c.has(i)) x[i] = to_float(row[c.at(i)]);
+    for (int i = 0; i < C; ++i) x[i] = 0.f;
+    if (c.vectors) {
+#pragma unroll
+      for (int i = 0; i < C; i += kVec)
+        if (c.has(i)) load_vector<T, kVec>(row + c.at(i), x + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i)
+        if (c.has(i)) x[i] = to_float(row[c.at(i)]);
+    }
   }
 }
 
@@ -202,6 +202,7 @@ __device__ __forceinline__ float sum_of(const Columns<C, kVec, kRing>& c, F term
 // Sums over the lanes of a row, for everyone: shuffles within a warp, then every thread adds the warps' sums in their
 // order.  Two exchanges in turn use the two halves of `part`: a warp that is through with one cannot reach the next but
 // one before all have left the first.  What lies behind the last warp's sums must be zero.
+template <int kThreads>
 struct RowSums {
   float (*part)[2][32];
   int lanes, turn;
@@ -222,7 +223,9 @@ struct RowSums {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       float s = 0.f;
-      for (int w = 0; w < lanes / 32; w += 4) {
+#pragma unroll
+      for (int w = 0; w < (kThreads + 31) / 32; w += 4) {
+        if (w >= 8 && w >= lanes / 32) break;
         const float4 q = *reinterpret_cast<const float4*>(&mine[k][w]);
         s += (q.x + q.y) + (q.z + q.w);
       }
@@ -238,8 +241,8 @@ __device__ __forceinline__ void clear_sums(float (*part)[2][32]) {
 }
 
 // x becomes x - mean; returns (mean, 1 / deviation).
-template <int C, int kVec, bool kRing>
-__device__ __forceinline__ float2 normalise(float (&x)[C], int kind, const Columns<C, kVec, kRing>& c, RowSums& sums, float eps) {
+template <int C, int kVec, bool kRing, typename S>
+__device__ __forceinline__ float2 normalise(float (&x)[C], int kind, const Columns<C, kVec, kRing>& c, S& sums, float eps) {
   const float per = 1.f / (float)c.channels;
   float mean = 0.f;
   if (kind == FBFFTCONV_NORM_LAYER) {
@@ -251,7 +254,7 @@ __device__ __forceinline__ float2 normalise(float (&x)[C], int kind, const Colum
   }
   float one[1] = {sum_of(c, [&](int i, float t) { return fmaf(x[i], x[i], t); })};
   sums(one);
-  return make_float2(mean, 1.f / sqrtf(fmaf(one[0], per, eps)));
+  return make_float2(mean, rsqrtf(fmaf(one[0], per, eps)));
 }
 
 __device__ __forceinline__ float sigmoid(float x) {
@@ -279,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 3 : kThreads <= 32
   grid_dependency_wait();
   const int slot = threadIdx.x / a.lanes, slots = blockDim.x / a.lanes;
   const Columns<C, kVec, kRing> c((int)threadIdx.x % a.lanes, a.lanes, a.channels, a.vectors);
-  RowSums sums{part, a.lanes, 0};
+  RowSums<kThreads> sums{part, a.lanes, 0};
   const int stride = gridDim.x * slots;
   const Ring<C, kVec, kRing> ring{staged + 16 * threadIdx.x, (2 * kT + kTR) * 16 * (int)blockDim.x, 16 * (int)blockDim.x, a.stages};
   const auto gate_row_of = [&](int row) { return a.per_gate == 1 ? row : row / a.per_gate; };
@@ -365,7 +368,7 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(const NormArgs 
   const int slots = blockDim.x / a.lanes;
   const int worker = blockIdx.x * slots + threadIdx.x / a.lanes, workers = gridDim.x * slots;
   const Columns<C, kVec, kRing> c((int)threadIdx.x % a.lanes, a.lanes, a.channels, a.vectors);
-  RowSums sums{part, a.lanes, 0};
+  RowSums<kThreads> sums{part, a.lanes, 0};
   const float per = 1.f / (float)a.channels;
   const bool shared_gate = kAll && a.gate_kind && a.per_gate > 1;
   // without shared gate rows all rows are one stretch, dealt out in turn; else `splits` workers deal out a gate row's

@@ -52,10 +52,11 @@ struct RecArgs {
   float* dstate0;        // or null
   float* sums;           // [part][channel] of dbias, or null
   long long rows, length, sequences;
-  long long x_stride, g_stride, z_stride, y_stride, dy_stride, dx_stride, dg_stride, dz_stride;
+  int x_stride, g_stride, z_stride, y_stride, dy_stride, dx_stride, dg_stride, dz_stride;
   long long per_segment; // sequences of a segment
   long long checkpoints_per_segment;
   int channels, wide_offsets, cluster;
+  bool wide;             // rows begin on 16 bytes
 };
 
 // Offsets of up to this many sequences are kept in shared memory: a search is a chain of loads.
@@ -259,39 +260,62 @@ template <typename T, int V> __device__ __forceinline__ void store_word(T* p, Ve
   else *p = from_float<T>(x.x);
 }
 
-// The words of a thread's next rows: in shared memory, on their way there while this round is computed.  A slot holds
-// one tensor's rows; it is filled anew as soon as the round has read it, one group of copies after the scan and one
-// after the outputs, so that the oldest group but one is always the one that is waited for.  Single 16-bit values,
-// which cp.async does not copy, are loaded where they are read.
+// The words of a warp's next rows: in shared memory, on their way there while this round is computed.  A slot holds
+// one tensor's rows, 128 bytes each; it is filled anew as soon as the round has read it, one group of copies after the
+// scan and one after the outputs, so that the oldest group but one is always the one that is waited for.  Where rows
+// begin on 16 bytes a lane copies such pieces of its warp's rows, past the L1 cache (`wide`; four times fewer copies,
+// and lines under way do not fill the cache: 131072 x 1024 forward took 487 us with words alone); else each its own
+// words.  Single 16-bit values, which cp.async does not copy, are loaded where they are read.
 template <typename T, int V, int kRows>
 struct Words {
   static constexpr bool kAsync = sizeof(T) * V == 4;
   static constexpr int kSlot = kRows * kThreads * 4;
-  char* base;  // this thread's
+  static constexpr int kPiece = 16 / sizeof(T);  // channels of a piece
+  char* base;      // this warp's
+  bool wide;
+  int channel, channels;  // of the warp's first lane; of a row
 
-  __device__ __forceinline__ void fetch(int slot, const T* p, long long stride, int n) const {
+  // `p`: the warp's channels of its first row
+  __device__ __forceinline__ void fetch(int slot, const T* p, int stride, int n) const {
     if constexpr (kAsync) {
+      const int lane = threadIdx.x & 31;
       const uint32_t to = (uint32_t)__cvta_generic_to_shared(base + slot * kSlot);
-      const auto copy = [&](auto all) {
+      if (wide) {
+        const int first = lane >> 3, piece = lane & 7;
+        const T* from = p + first * stride + piece * kPiece;
+        const uint32_t at = to + first * 128 + piece * 16;
+        const int rows = channel + piece * kPiece < channels ? n : 0;
+#pragma unroll
+        for (int i = 0; i < kRows; i += 4)
+          if (first + i < rows)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + i * 128), "l"(from + i * stride) : "memory");
+      } else {
+        const T* from = p + lane * V;
+        const int rows = channel + lane * V < channels ? n : 0;
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
-          if (all || i < n)
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + i * kThreads * 4), "l"(p + i * stride) : "memory");
-      };
-      if (n == kRows) copy(std::true_type{});
-      else copy(std::false_type{});
+          if (i < rows)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + i * 128 + lane * 4), "l"(from + i * stride) : "memory");
+      }
     }
   }
   __device__ __forceinline__ void commit() const {
     if constexpr (kAsync) asm volatile("cp.async.commit_group;" ::: "memory");
   }
   __device__ __forceinline__ void wait() const {
-    if constexpr (kAsync) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    if constexpr (kAsync) {
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      __syncwarp();
+    }
+  }
+  // before a slot is filled anew: every lane has read it
+  __device__ __forceinline__ void release() const {
+    if constexpr (kAsync) __syncwarp();
   }
   // row i of the slot, which is that of `p`
-  __device__ __forceinline__ Vec<V> read(int slot, const T* p, long long stride, int i) const {
-    if constexpr (kAsync) return unpack<T, V>(*reinterpret_cast<const uint32_t*>(base + slot * kSlot + i * kThreads * 4));
-    else return unpack<T, V>(load_word<T, V>(p + i * stride));
+  __device__ __forceinline__ Vec<V> read(int slot, const T* p, int stride, int i) const {
+    if constexpr (kAsync) return unpack<T, V>(*reinterpret_cast<const uint32_t*>(base + slot * kSlot + i * 128 + (threadIdx.x & 31) * 4));
+    else return unpack<T, V>(load_word<T, V>(p + (channel + (threadIdx.x & 31) * V < channels ? (threadIdx.x & 31) * V : 0) + i * stride));
   }
 };
 
@@ -434,26 +458,29 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const _
   segment_rows(a, kept, begin, end);
   if (rank == 0) pass_empty<V>(a, kept, a.state0, a.state, c, on);
   const long long tiles = (end - begin + kTile - 1) / kTile, rounds = (tiles + blocks - 1) / blocks;
-  const Words<T, V, L> words{staged + 4 * threadIdx.x};
+  const int group = blockIdx.x / blocks * 32 * V;  // the first lane's channel
+  const Words<T, V, L> words{staged + warp * (L * 128), a.wide, group, a.channels};
   enum { kX, kG, kZ };  // slots
-  const T* const x0 = static_cast<const T*>(a.x) + c;
-  const T* const g0 = static_cast<const T*>(a.g) + c;
-  const T* const z0 = static_cast<const T*>(a.z) + c;
+  const T* const x0 = static_cast<const T*>(a.x) + group;
+  const T* const g0 = static_cast<const T*>(a.g) + group;
+  const T* const z0 = static_cast<const T*>(a.z) + group;
   const Vec<V> bias = a.bias ? load_floats<V>(a.bias + c) : all_of<V>(0.f);
   Vec<V> carry = all_of<V>(0.f);
   start_exchange(shared, blocks);
   const auto row_of = [&](long long round) { return begin + ((round * blocks + rank) * kWarps + warp) * L; };
   const auto rows_at = [&](long long row) { return (int)max(0ll, min((long long)L, end - row)); };
   const auto fetch_inputs = [&](long long round) {
+    words.release();
     const long long row = row_of(round);
-    const int n = on ? rows_at(row) : 0;
+    const int n = rows_at(row);
     words.fetch(kX, x0 + row * a.x_stride, a.x_stride, n);
     words.fetch(kG, g0 + row * a.g_stride, a.g_stride, n);
     words.commit();
   };
   const auto fetch_outputs = [&](long long round) {
+    words.release();
     const long long row = row_of(round);
-    if (kGate) words.fetch(kZ, z0 + row * a.z_stride, a.z_stride, on ? rows_at(row) : 0);
+    if (kGate) words.fetch(kZ, z0 + row * a.z_stride, a.z_stride, rows_at(row));
     words.commit();
   };
   fetch_inputs(0);
@@ -536,12 +563,13 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
   segment_rows(a, kept, begin, end);
   if (rank == 0) pass_empty<V>(a, kept, a.dstate, a.dstate0, c, on);
   const long long tiles = (end - begin + kTile - 1) / kTile, rounds = (tiles + blocks - 1) / blocks;
-  const Words<T, V, L> words{staged + 4 * threadIdx.x};
+  const int group = blockIdx.x / blocks * 32 * V;  // the first lane's channel
+  const Words<T, V, L> words{staged + warp * (L * 128), a.wide, group, a.channels};
   enum { kX, kG = 2, kDy, kZ };  // slots: x has two, it is read to the end of its round
-  const T* const x0 = static_cast<const T*>(a.x) + c;
-  const T* const g0 = static_cast<const T*>(a.g) + c;
-  const T* const dy0 = static_cast<const T*>(a.dy) + c;
-  const T* const z0 = static_cast<const T*>(a.z) + c;
+  const T* const x0 = static_cast<const T*>(a.x) + group;
+  const T* const g0 = static_cast<const T*>(a.g) + group;
+  const T* const dy0 = static_cast<const T*>(a.dy) + group;
+  const T* const z0 = static_cast<const T*>(a.z) + group;
   const Vec<V> bias = a.bias ? load_floats<V>(a.bias + c) : all_of<V>(0.f);
   Vec<V> carry = all_of<V>(0.f), dbias = all_of<V>(0.f);
   start_exchange(shared, blocks);
@@ -550,15 +578,17 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
   const auto row_of = [&](long long round) { return begin + (tile_of(round) * kWarps + warp) * L; };
   const auto rows_at = [&](long long round) { return tile_of(round) < 0 ? 0 : (int)max(0ll, min((long long)L, end - row_of(round))); };
   const auto fetch_inputs = [&](long long round) {
+    words.release();
     const long long row = row_of(round);
-    const int n = on ? rows_at(round) : 0;
+    const int n = rows_at(round);
     words.fetch(kX + (int)(round & 1), x0 + row * a.x_stride, a.x_stride, n);
     words.fetch(kG, g0 + row * a.g_stride, a.g_stride, n);
     words.commit();
   };
   const auto fetch_outputs = [&](long long round) {
+    words.release();
     const long long row = row_of(round);
-    const int n = on ? rows_at(round) : 0;
+    const int n = rows_at(round);
     words.fetch(kDy, dy0 + row * a.dy_stride, a.dy_stride, n);
     if (kGate) words.fetch(kZ, z0 + row * a.z_stride, a.z_stride, n);
     words.commit();
@@ -831,6 +861,10 @@ int check_desc(const fbfftconv_recurrence_desc* d) {
   if (d->sequences < 0 || d->length < 0 || d->rows < 0) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "negative size");
   if (d->sequences > (1ll << 31) || d->length > (1ll << 40) || d->rows > (1ll << 40))
     return op_fail(FBFFTCONV_ERR_UNSUPPORTED_SIZE, "more than 2^31 sequences or 2^40 rows");
+  const int64_t strides[] = {d->x_stride, d->g_stride, d->z_stride, d->y_stride, d->grad_y_stride, d->grad_x_stride,
+                             d->grad_g_stride, d->grad_z_stride};
+  for (const int64_t s : strides)
+    if (s > (1ll << 26)) return op_fail(FBFFTCONV_ERR_UNSUPPORTED_SIZE, "more than 2^26 elements between rows");
   if (!known_type(d->type)) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "unknown element type");
   if (!d->offsets && ((d->length > 0 && d->sequences > d->rows / d->length) || d->rows != d->sequences * d->length))
     return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "rows are not sequences times length");
@@ -848,13 +882,16 @@ struct RowPointer {
 
 template <int N, int M>
 int check_rec_pointers(const RowPointer (&rows)[N], const RowPointer (&floats)[M], const fbfftconv_recurrence_desc& d,
-                       int device, bool* pairs) {
+                       int device, bool* pairs, bool* wide) {
+  const int piece = 16 / type_bytes(d.type);
   *pairs = d.channels % 2 == 0;
+  *wide = d.channels % piece == 0;
   for (const RowPointer& q : rows) {
     if (!q.p && q.needed) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "%s is null", q.name);
     if (!aligned_to(q.p, type_bytes(d.type))) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "%s is not aligned to its element", q.name);
     if (q.p && q.stride < d.channels) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "the rows of %s overlap", q.name);
     if (q.p && (q.stride % 2 || !aligned_to(q.p, 2 * type_bytes(d.type)))) *pairs = false;
+    if (q.p && (q.stride % piece || !aligned_to(q.p, 16))) *wide = false;
   }
   for (const RowPointer& q : floats) {
     if (!q.p && q.needed) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "%s is null", q.name);
@@ -866,7 +903,7 @@ int check_rec_pointers(const RowPointer (&rows)[N], const RowPointer (&floats)[M
 }
 
 RecArgs common_args(const fbfftconv_recurrence_desc& d) {
-  const auto or_dense = [&](int64_t s) { return s ? (long long)s : (long long)d.channels; };
+  const auto or_dense = [&](int64_t s) { return s ? (int)s : d.channels; };
   RecArgs a{};
   a.rows = d.rows, a.length = d.length, a.sequences = d.sequences, a.channels = d.channels;
   a.offsets = d.offsets, a.wide_offsets = d.wide_offsets;
@@ -925,7 +962,7 @@ int fbfftconv_recurrence(const fbfftconv_recurrence_desc* desc, const void* x, c
   if (state0 && state0 == state && d.sequences > 0)
     return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "the final state must not overwrite the initial one");
   OP_TRY(resolve_device(d.device, &device));
-  OP_TRY(check_rec_pointers(rows, floats, d, device, &pairs));
+  OP_TRY(check_rec_pointers(rows, floats, d, device, &pairs, &a.wide));
   if (d.sequences == 0) return FBFFTCONV_OK;
   const OnDevice on(device);
   if (on.error() != cudaSuccess) return op_cuda_fail(on.error(), "cudaSetDevice");
@@ -961,7 +998,7 @@ int fbfftconv_recurrence_backward(const fbfftconv_recurrence_desc* desc, const v
   if (grad_state && grad_state == grad_state0 && d.sequences > 0)
     return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "the states' gradients must not share memory");
   OP_TRY(resolve_device(d.device, &device));
-  OP_TRY(check_rec_pointers(rows, floats, d, device, &pairs));
+  OP_TRY(check_rec_pointers(rows, floats, d, device, &pairs, &a.wide));
   const OnDevice on(device);
   if (on.error() != cudaSuccess) return op_cuda_fail(on.error(), "cudaSetDevice");
   const Division s = division_for(d, pairs);
@@ -1027,7 +1064,7 @@ int fbfftconv_recurrence_step(const fbfftconv_recurrence_desc* desc, const void*
   int device;
   bool pairs;
   OP_TRY(resolve_device(d.device, &device));
-  OP_TRY(check_rec_pointers(rows, floats, d, device, &pairs));
+  OP_TRY(check_rec_pointers(rows, floats, d, device, &pairs, &a.wide));
   if (!some) return FBFFTCONV_OK;
   const OnDevice on(device);
   if (on.error() != cudaSuccess) return op_cuda_fail(on.error(), "cudaSetDevice");

@@ -360,7 +360,7 @@ int fbfftconv_adamw_step(fbfftconv_adamw* h, double lr, float grad_scale, const 
 /* ---- gated linear recurrence along sequences -------------------------------------------------
  *   a_t = sigmoid(g_t + bias),  h_t = a_t h_{t-1} + (1 - a_t) x_t,  y_t = h_t silu(z_t)   (y_t = h_t where z is null)
  * with h_{-1} the sequence's initial state (zero where state0 is null).  x, g, z, y are rows of `channels` neighbours of
- * one type, their stride (elements; 0 = channels) apart; bias (channels), states (sequences, channels) and checkpoints
+ * one type, their stride (elements, at most 2^26; 0 = channels) apart; bias (channels), states (sequences, channels) and checkpoints
  * are fp32.  The rows are those of `sequences` sequences of `length` rows one behind the other (rows = sequences *
  * length), or, with offsets (sequences + 1 integers on the device, 32 or with wide_offsets 64 bits wide, not falling),
  * sequence i has rows [offsets[i], offsets[i + 1]) of `rows`; rows outside of all sequences are neither read nor

@@ -30,6 +30,7 @@ constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kForwardRows = 16, kBackwardRows = 8;  // of a warp, in a round
 constexpr int kCheckpoint = 64;                      // rows between the states that forward leaves for backward
 constexpr int kMostCluster = 16;
+constexpr long long kMostRows = 1ll << 30;             // rows are 32 bits wide in the kernels
 static_assert(kCheckpoint % kForwardRows == 0 && kWarps * kBackwardRows == kCheckpoint && (kWarps * kForwardRows) % kCheckpoint == 0);
 
 struct RecArgs {
@@ -51,10 +52,10 @@ struct RecArgs {
   void* dz;
   float* dstate0;        // or null
   float* sums;           // [part][channel] of dbias, or null
-  long long rows, length, sequences;
+  int rows, length, sequences;
   int x_stride, g_stride, z_stride, y_stride, dy_stride, dx_stride, dg_stride, dz_stride;
-  long long per_segment; // sequences of a segment
-  long long checkpoints_per_segment;
+  int per_segment;       // sequences of a segment
+  int checkpoints_per_segment;
   int channels, wide_offsets, cluster;
   bool wide;             // rows begin on 16 bytes
 };
@@ -62,15 +63,15 @@ struct RecArgs {
 // Offsets of up to this many sequences are kept in shared memory: a search is a chain of loads.
 constexpr int kKeptOffsets = 512;
 
-__device__ __forceinline__ long long load_offset(const RecArgs& a, long long i) {
+__device__ __forceinline__ int load_offset(const RecArgs& a, int i) {
   const long long v = a.wide_offsets ? static_cast<const long long*>(a.offsets)[i] : static_cast<const int*>(a.offsets)[i];
-  return v < 0 ? 0 : v > a.rows ? a.rows : v;  // a bad offset must not lead out of the tensors
+  return (int)(v < 0 ? 0 : v > a.rows ? a.rows : v);  // a bad offset must not lead out of the tensors
 }
 
-__device__ __forceinline__ long long offset_at(const RecArgs& a, const long long* kept, long long i) {
+__device__ __forceinline__ int offset_at(const RecArgs& a, const int* kept, int i) {
   return a.sequences <= kKeptOffsets ? kept[i] : load_offset(a, i);
 }
-__device__ __forceinline__ void keep_offsets(const RecArgs& a, long long* kept) {
+__device__ __forceinline__ void keep_offsets(const RecArgs& a, int* kept) {
   if (a.offsets && a.sequences <= kKeptOffsets)
     for (int i = threadIdx.x; i <= a.sequences; i += kThreads) kept[i] = load_offset(a, i);
   __syncthreads();
@@ -78,16 +79,16 @@ __device__ __forceinline__ void keep_offsets(const RecArgs& a, long long* kept) 
 
 // The sequence that a row belongs to, and the rows where it begins and ends.
 struct Sequence {
-  long long index, begin, end;
+  int index, begin, end;
 };
-__device__ __forceinline__ Sequence sequence_of(const RecArgs& a, const long long* kept, long long row) {
+__device__ __forceinline__ Sequence sequence_of(const RecArgs& a, const int* kept, int row) {
   if (!a.offsets) {
-    const long long i = (a.rows | a.length) >> 32 ? row / a.length : (uint32_t)row / (uint32_t)a.length;
+    const int i = row / a.length;
     return {i, i * a.length, (i + 1) * a.length};
   }
-  long long lo = 0, hi = a.sequences;  // the last one that begins at or before the row
+  int lo = 0, hi = a.sequences;  // the last one that begins at or before the row
   while (hi - lo > 1) {
-    const long long mid = (lo + hi) >> 1;
+    const int mid = (lo + hi) >> 1;
     if (offset_at(a, kept, mid) <= row) lo = mid;
     else hi = mid;
   }
@@ -95,21 +96,21 @@ __device__ __forceinline__ Sequence sequence_of(const RecArgs& a, const long lon
 }
 
 // The sequence that a row belongs to, for the few rows that begin or end one: kept out of the loops' code.
-__device__ __noinline__ long long index_of(const RecArgs& a, const long long* kept, long long row) { return sequence_of(a, kept, row).index; }
+__device__ __noinline__ int index_of(const RecArgs& a, const int* kept, int row) { return sequence_of(a, kept, row).index; }
 
 // Which of a warp's rows begin a sequence, and which end one.  `in`, the sequence that its rows were in last, is looked
 // up anew only where they have left it; most rounds lie within one sequence.
 struct Borders {
   uint32_t first, last;
 };
-__device__ __forceinline__ Borders borders(const RecArgs& a, const long long* kept, long long row, int n, Sequence& in) {
+__device__ __forceinline__ Borders borders(const RecArgs& a, const int* kept, int row, int n, Sequence& in) {
   Borders b{0, 0};
   if (n <= 0) return b;
   if (row < in.begin || row >= in.end) in = sequence_of(a, kept, row);
   if (row > in.begin && in.end - row > n) return b;
   if (row == in.begin) b.first = 1;
   while (in.end > row && in.end - row <= n) {
-    const int k = (int)(in.end - row);
+    const int k = in.end - row;
     b.last |= 1u << (k - 1);
     if (k == n) break;
     b.first |= 1u << k;
@@ -418,26 +419,26 @@ __global__ void wait_probe_kernel(int* gave_up) {
 }
 
 // The rows of this block's segment: [begin, end).
-__device__ __forceinline__ void segment_rows(const RecArgs& a, const long long* kept, long long& begin, long long& end) {
+__device__ __forceinline__ void segment_rows(const RecArgs& a, const int* kept, int& begin, int& end) {
   if (a.offsets) {
     begin = offset_at(a, kept, 0);
     end = offset_at(a, kept, a.sequences);
   } else {
-    const long long first = (long long)blockIdx.y * a.per_segment;
-    const long long last = min(first + a.per_segment, a.sequences);
+    const int first = blockIdx.y * a.per_segment;
+    const int last = min(first + a.per_segment, a.sequences);
     begin = first * a.length, end = last * a.length;
   }
 }
 
 // Sequences without rows hand their state on.
 template <int V>
-__device__ __forceinline__ void pass_empty(const RecArgs& a, const long long* kept, const float* from, float* to, int channel, bool on) {
+__device__ __forceinline__ void pass_empty(const RecArgs& a, const int* kept, const float* from, float* to, int channel, bool on) {
   if (!to || blockIdx.y || (!a.offsets && a.length > 0)) return;
-  for (long long s = threadIdx.x >> 5; s < a.sequences; s += kWarps) {
+  for (int s = threadIdx.x >> 5; s < a.sequences; s += kWarps) {
     if (a.offsets && offset_at(a, kept, s + 1) > offset_at(a, kept, s)) continue;
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      if (on) to[s * a.channels + channel + v] = from ? from[s * a.channels + channel + v] : 0.f;
+      if (on) to[(long long)s * a.channels + channel + v] = from ? from[(long long)s * a.channels + channel + v] : 0.f;
   }
 }
 
@@ -446,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const _
   constexpr int L = kForwardRows, kTile = kWarps * L;
   extern __shared__ __align__(16) char staged[];
   __shared__ __align__(16) Exchange<V> shared;
-  __shared__ long long kept[kKeptOffsets + 1];
+  __shared__ int kept[kKeptOffsets + 1];
   grid_dependency_wait();
   keep_offsets(a, kept);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -454,10 +455,10 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const _
   const int channel = (blockIdx.x / blocks * 32 + lane) * V;
   const bool on = channel < a.channels;
   const int c = on ? channel : 0;
-  long long begin, end;
+  int begin, end;
   segment_rows(a, kept, begin, end);
   if (rank == 0) pass_empty<V>(a, kept, a.state0, a.state, c, on);
-  const long long tiles = (end - begin + kTile - 1) / kTile, rounds = (tiles + blocks - 1) / blocks;
+  const int tiles = (end - begin + kTile - 1) / kTile, rounds = (tiles + blocks - 1) / blocks;
   const int group = blockIdx.x / blocks * 32 * V;  // the first lane's channel
   const Words<T, V, L> words{staged + warp * (L * 128), a.wide, group, a.channels};
   enum { kX, kG, kZ };  // slots
@@ -467,31 +468,31 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const _
   const Vec<V> bias = a.bias ? load_floats<V>(a.bias + c) : all_of<V>(0.f);
   Vec<V> carry = all_of<V>(0.f);
   start_exchange(shared, blocks);
-  const auto row_of = [&](long long round) { return begin + ((round * blocks + rank) * kWarps + warp) * L; };
-  const auto rows_at = [&](long long row) { return (int)max(0ll, min((long long)L, end - row)); };
-  const auto fetch_inputs = [&](long long round) {
+  const auto row_of = [&](int round) { return begin + ((round * blocks + rank) * kWarps + warp) * L; };
+  const auto rows_at = [&](int row) { return max(0, min(L, end - row)); };
+  const auto fetch_inputs = [&](int round) {
     words.release();
-    const long long row = row_of(round);
+    const int row = row_of(round);
     const int n = rows_at(row);
-    words.fetch(kX, x0 + row * a.x_stride, a.x_stride, n);
-    words.fetch(kG, g0 + row * a.g_stride, a.g_stride, n);
+    words.fetch(kX, x0 + (long long)row * a.x_stride, a.x_stride, n);
+    words.fetch(kG, g0 + (long long)row * a.g_stride, a.g_stride, n);
     words.commit();
   };
-  const auto fetch_outputs = [&](long long round) {
+  const auto fetch_outputs = [&](int round) {
     words.release();
-    const long long row = row_of(round);
-    if (kGate) words.fetch(kZ, z0 + row * a.z_stride, a.z_stride, rows_at(row));
+    const int row = row_of(round);
+    if (kGate) words.fetch(kZ, z0 + (long long)row * a.z_stride, a.z_stride, rows_at(row));
     words.commit();
   };
   fetch_inputs(0);
   fetch_outputs(0);
   Sequence in{0, 0, 0};
-  for (long long round = 0; round < rounds; ++round) {
-    const long long row = row_of(round);
+  for (int round = 0; round < rounds; ++round) {
+    const int row = row_of(round);
     const int n = rows_at(row);
-    const T* const xs = x0 + row * a.x_stride;
-    const T* const gs = g0 + row * a.g_stride;
-    const T* const zs = z0 + row * a.z_stride;
+    const T* const xs = x0 + (long long)row * a.x_stride;
+    const T* const gs = g0 + (long long)row * a.g_stride;
+    const T* const zs = z0 + (long long)row * a.z_stride;
     words.wait();
     const Borders at = borders(a, kept, row, n, in);
     const bool within = n == L && at.first == 0 && at.last == 0;  // all rows there, none at a sequence's border
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const _
           gate_of(words.read(kG, gs, a.g_stride, i) + bias, A[i], B[i]);
           B[i] = B[i] * words.read(kX, xs, a.x_stride, i);
           if (!plain && (at.first >> i & 1)) {  // the row takes the initial state, whatever comes before it
-            if (a.state0) B[i] = fma(A[i], load_floats<V>(a.state0 + index_of(a, kept, row + i) * a.channels + c), B[i]);
+            if (a.state0) B[i] = fma(A[i], load_floats<V>(a.state0 + (long long)index_of(a, kept, row + i) * a.channels + c), B[i]);
             mine = Stretch<V>{all_of<V>(-1.f), B[i]};
           } else {
             const bool cut = !plain && mine.A.x < 0.f;
@@ -521,8 +522,8 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const _
     Vec<V> h = exchange(shared, (uint32_t)round, warp, rank, blocks, mine, carry);
     words.wait();
     if (a.checkpoints && n > 0 && on && (row - begin) % kCheckpoint == 0)
-      store_floats(a.checkpoints + (blockIdx.y * a.checkpoints_per_segment + (row - begin) / kCheckpoint) * a.channels + c, h);
-    T* y = static_cast<T*>(a.y) + row * a.y_stride + c;
+      store_floats(a.checkpoints + (long long)(blockIdx.y * a.checkpoints_per_segment + (row - begin) / kCheckpoint) * a.channels + c, h);
+    T* y = static_cast<T*>(a.y) + (long long)row * a.y_stride + c;
     const auto emit = [&](auto plain) {
 #pragma unroll
       for (int i = 0; i < L; ++i) {
@@ -536,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const _
         }
         if (on) store_word<T, V>(y + i * a.y_stride, out);
         if (!plain && (at.last >> i & 1) && a.state && on)
-          store_floats(a.state + index_of(a, kept, row + i) * a.channels + c, h);
+          store_floats(a.state + (long long)index_of(a, kept, row + i) * a.channels + c, h);
       }
     };
     if (within) emit(std::true_type{});
@@ -551,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
   extern __shared__ __align__(16) char staged[];
   __shared__ __align__(16) Exchange<V> shared;
   __shared__ Stretch<V> states[2][kWarps][32];
-  __shared__ long long kept[kKeptOffsets + 1];
+  __shared__ int kept[kKeptOffsets + 1];
   grid_dependency_wait();
   keep_offsets(a, kept);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -559,10 +560,10 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
   const int channel = (blockIdx.x / blocks * 32 + lane) * V;
   const bool on = channel < a.channels;
   const int c = on ? channel : 0;
-  long long begin, end;
+  int begin, end;
   segment_rows(a, kept, begin, end);
   if (rank == 0) pass_empty<V>(a, kept, a.dstate, a.dstate0, c, on);
-  const long long tiles = (end - begin + kTile - 1) / kTile, rounds = (tiles + blocks - 1) / blocks;
+  const int tiles = (end - begin + kTile - 1) / kTile, rounds = (tiles + blocks - 1) / blocks;
   const int group = blockIdx.x / blocks * 32 * V;  // the first lane's channel
   const Words<T, V, L> words{staged + warp * (L * 128), a.wide, group, a.channels};
   enum { kX, kG = 2, kDy, kZ };  // slots: x has two, it is read to the end of its round
@@ -574,39 +575,39 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
   Vec<V> carry = all_of<V>(0.f), dbias = all_of<V>(0.f);
   start_exchange(shared, blocks);
   // the last rows come first
-  const auto tile_of = [&](long long round) { return tiles - 1 - (round * blocks + rank); };
-  const auto row_of = [&](long long round) { return begin + (tile_of(round) * kWarps + warp) * L; };
-  const auto rows_at = [&](long long round) { return tile_of(round) < 0 ? 0 : (int)max(0ll, min((long long)L, end - row_of(round))); };
-  const auto fetch_inputs = [&](long long round) {
+  const auto tile_of = [&](int round) { return tiles - 1 - (round * blocks + rank); };
+  const auto row_of = [&](int round) { return begin + (tile_of(round) * kWarps + warp) * L; };
+  const auto rows_at = [&](int round) { return tile_of(round) < 0 ? 0 : max(0, min(L, end - row_of(round))); };
+  const auto fetch_inputs = [&](int round) {
     words.release();
-    const long long row = row_of(round);
+    const int row = row_of(round);
     const int n = rows_at(round);
-    words.fetch(kX + (int)(round & 1), x0 + row * a.x_stride, a.x_stride, n);
-    words.fetch(kG, g0 + row * a.g_stride, a.g_stride, n);
+    words.fetch(kX + (int)(round & 1), x0 + (long long)row * a.x_stride, a.x_stride, n);
+    words.fetch(kG, g0 + (long long)row * a.g_stride, a.g_stride, n);
     words.commit();
   };
-  const auto fetch_outputs = [&](long long round) {
+  const auto fetch_outputs = [&](int round) {
     words.release();
-    const long long row = row_of(round);
+    const int row = row_of(round);
     const int n = rows_at(round);
-    words.fetch(kDy, dy0 + row * a.dy_stride, a.dy_stride, n);
-    if (kGate) words.fetch(kZ, z0 + row * a.z_stride, a.z_stride, n);
+    words.fetch(kDy, dy0 + (long long)row * a.dy_stride, a.dy_stride, n);
+    if (kGate) words.fetch(kZ, z0 + (long long)row * a.z_stride, a.z_stride, n);
     words.commit();
   };
   fetch_inputs(0);
   fetch_outputs(0);
   Sequence in{0, 0, 0};
-  for (long long round = 0; round < rounds; ++round) {
+  for (int round = 0; round < rounds; ++round) {
     const int stage = (int)(round & 1);
-    const long long row = row_of(round), tile = tile_of(round);
+    const int row = row_of(round), tile = tile_of(round);
     const int n = rows_at(round);
-    const T* const xs = x0 + row * a.x_stride;
-    const T* const gs = g0 + row * a.g_stride;
-    const T* const dys = dy0 + row * a.dy_stride;
-    const T* const zs = z0 + row * a.z_stride;
+    const T* const xs = x0 + (long long)row * a.x_stride;
+    const T* const gs = g0 + (long long)row * a.g_stride;
+    const T* const dys = dy0 + (long long)row * a.dy_stride;
+    const T* const zs = z0 + (long long)row * a.z_stride;
     // the state before the tile
     Vec<V> h = tile < 0 ? all_of<V>(0.f)
-                        : load_floats<V>(a.checkpoints + (blockIdx.y * a.checkpoints_per_segment + tile) * a.channels + c);
+                        : load_floats<V>(a.checkpoints + (long long)(blockIdx.y * a.checkpoints_per_segment + tile) * a.channels + c);
     words.wait();
     const Borders at = borders(a, kept, row, n, in);
     const bool within = n == L && at.first == 0 && at.last == 0;  // all rows there, none at a sequence's border
@@ -620,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
           gate_of(words.read(kG, gs, a.g_stride, i) + bias, A[i], B[i]);
           const Vec<V> in_x = B[i] * words.read(kX + stage, xs, a.x_stride, i);
           if (!plain && (at.first >> i & 1)) {
-            P[i] = a.state0 ? load_floats<V>(a.state0 + index_of(a, kept, row + i) * a.channels + c) : all_of<V>(0.f);
+            P[i] = a.state0 ? load_floats<V>(a.state0 + (long long)index_of(a, kept, row + i) * a.channels + c) : all_of<V>(0.f);
             mine = Stretch<V>{all_of<V>(-1.f), fma(A[i], P[i], in_x)};
           } else {
             const bool cut = !plain && mine.A.x < 0.f;
@@ -638,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
     __syncthreads();
     for (int w = 0; w < warp; ++w) h = apply(states[stage][w][lane], h);
     words.wait();
-    T* dz = static_cast<T*>(a.dz) + row * a.dz_stride + c;
+    T* dz = static_cast<T*>(a.dz) + (long long)row * a.dz_stride + c;
     // forward from row to row; then back, what flows to the rows before: d -> A (E + d), nothing across the beginning
     // of a sequence
     mine = nothing<V>();
@@ -660,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
           if (a.dz && on) store_word<T, V>(dz + i * a.dz_stride, (ds * h) * slope);
         }
         if (!plain && (at.last >> i & 1) && a.dstate)
-          E[i] = E[i] + load_floats<V>(a.dstate + index_of(a, kept, row + i) * a.channels + c);
+          E[i] = E[i] + load_floats<V>(a.dstate + (long long)index_of(a, kept, row + i) * a.channels + c);
       }
 #pragma unroll
       for (int i = L - 1; i >= 0; --i) {
@@ -674,8 +675,8 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
     else through(std::false_type{});
     fetch_outputs(round + 1);
     Vec<V> d = exchange(shared, (uint32_t)round, kWarps - 1 - warp, rank, blocks, mine, carry);
-    T* dx = static_cast<T*>(a.dx) + row * a.dx_stride + c;
-    T* dg = static_cast<T*>(a.dg) + row * a.dg_stride + c;
+    T* dx = static_cast<T*>(a.dx) + (long long)row * a.dx_stride + c;
+    T* dg = static_cast<T*>(a.dg) + (long long)row * a.dg_stride + c;
     const auto emit = [&](auto plain) {
 #pragma unroll
       for (int i = L - 1; i >= 0; --i) {
@@ -689,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
         if (a.dx && on) store_word<T, V>(dx + i * a.dx_stride, out);
         if (a.dg && on) store_word<T, V>(dg + i * a.dg_stride, gate);
         if (!plain && (at.first >> i & 1)) {
-          if (a.dstate0 && on) store_floats(a.dstate0 + index_of(a, kept, row + i) * a.channels + c, d);
+          if (a.dstate0 && on) store_floats(a.dstate0 + (long long)index_of(a, kept, row + i) * a.channels + c, d);
           d = all_of<V>(0.f);
         }
       }
@@ -859,8 +860,8 @@ int check_desc(const fbfftconv_recurrence_desc* d) {
   if (!d) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "null argument");
   if (d->channels <= 0 || d->channels > (1 << 22)) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "1 to 2^22 channels");
   if (d->sequences < 0 || d->length < 0 || d->rows < 0) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "negative size");
-  if (d->sequences > (1ll << 31) || d->length > (1ll << 40) || d->rows > (1ll << 40))
-    return op_fail(FBFFTCONV_ERR_UNSUPPORTED_SIZE, "more than 2^31 sequences or 2^40 rows");
+  if (d->sequences > kMostRows || d->length > kMostRows || d->rows > kMostRows)
+    return op_fail(FBFFTCONV_ERR_UNSUPPORTED_SIZE, "more than 2^30 sequences or rows");
   const int64_t strides[] = {d->x_stride, d->g_stride, d->z_stride, d->y_stride, d->grad_y_stride, d->grad_x_stride,
                              d->grad_g_stride, d->grad_z_stride};
   for (const int64_t s : strides)
@@ -905,7 +906,7 @@ int check_rec_pointers(const RowPointer (&rows)[N], const RowPointer (&floats)[M
 RecArgs common_args(const fbfftconv_recurrence_desc& d) {
   const auto or_dense = [&](int64_t s) { return s ? (int)s : d.channels; };
   RecArgs a{};
-  a.rows = d.rows, a.length = d.length, a.sequences = d.sequences, a.channels = d.channels;
+  a.rows = (int)d.rows, a.length = (int)d.length, a.sequences = (int)d.sequences, a.channels = d.channels;
   a.offsets = d.offsets, a.wide_offsets = d.wide_offsets;
   a.x_stride = or_dense(d.x_stride), a.g_stride = or_dense(d.g_stride), a.z_stride = or_dense(d.z_stride);
   a.y_stride = or_dense(d.y_stride), a.dy_stride = or_dense(d.grad_y_stride);
@@ -968,7 +969,7 @@ int fbfftconv_recurrence(const fbfftconv_recurrence_desc* desc, const void* x, c
   if (on.error() != cudaSuccess) return op_cuda_fail(on.error(), "cudaSetDevice");
   const Division s = division_for(d, pairs);
   a.x = x, a.g = g, a.z = z, a.bias = bias, a.state0 = state0, a.y = y, a.state = state, a.checkpoints = checkpoints;
-  a.per_segment = s.per_segment, a.checkpoints_per_segment = s.checkpoints;
+  a.per_segment = (int)s.per_segment, a.checkpoints_per_segment = (int)s.checkpoints;
   count_launch();
 #define FORWARD(T, V) forward<T, V>(a, s, static_cast<cudaStream_t>(stream))
   const cudaError_t e = BY_TYPE(FORWARD);
@@ -1010,7 +1011,7 @@ int fbfftconv_recurrence_backward(const fbfftconv_recurrence_desc* desc, const v
     a.x = x, a.g = g, a.z = z, a.bias = bias, a.state0 = state0, a.checkpoints = const_cast<float*>(checkpoints);
     a.dy = grad_y, a.dstate = grad_state, a.dx = grad_x, a.dg = grad_g, a.dz = grad_z, a.dstate0 = grad_state0;
     a.sums = grad_bias ? static_cast<float*>(workspace) : nullptr;
-    a.per_segment = s.per_segment, a.checkpoints_per_segment = s.checkpoints;
+    a.per_segment = (int)s.per_segment, a.checkpoints_per_segment = (int)s.checkpoints;
     count_launch();
 #define BACKWARD(T, V) backward<T, V>(a, s, &parts, cuda_stream)
     const cudaError_t e = BY_TYPE(BACKWARD);

@@ -364,7 +364,8 @@ int fbfftconv_adamw_step(fbfftconv_adamw* h, double lr, float grad_scale, const 
  * are fp32.  The rows are those of `sequences` sequences of `length` rows one behind the other (rows = sequences *
  * length), or, with offsets (sequences + 1 integers on the device, 32 or with wide_offsets 64 bits wide, not falling),
  * sequence i has rows [offsets[i], offsets[i + 1]) of `rows`; rows outside of all sequences are neither read nor
- * written.  Sequences may be empty: their state passes through.  Nothing of a sequence, not even a NaN, reaches the
+ * written.  Sequences may be empty: their state passes through.  At most
+ * 2^30 rows and sequences.  Nothing of a sequence, not even a NaN, reaches the
  * next.  Results do not depend on the timing of blocks: the same call gives the same bits. */
 typedef struct fbfftconv_recurrence_desc {
   int64_t rows, sequences, length;

@@ -163,23 +163,31 @@ __device__ __forceinline__ void load_codes(const uint8_t* base, long long at, in
   }
 }
 
-// The first moment's code is the lowest byte of c, the second's the one above.
+// Four codes, the lowest bytes of c, with the signs of x.
+__device__ __forceinline__ uint32_t pack_codes(const uint32_t* c) {
+  return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+}
+__device__ __forceinline__ uint32_t pack_codes(const uint32_t* c, const float* x) {
+  const uint32_t a = __byte_perm(__float_as_uint(x[0]), __float_as_uint(x[1]), 0x0073);
+  const uint32_t b = __byte_perm(__float_as_uint(x[2]), __float_as_uint(x[3]), 0x0073);
+  return pack_codes(c) | (__byte_perm(a, b, 0x5410) & 0x80808080u);
+}
+
+// The codes of both moments, the first's with the signs of m.
 template <bool kVectors>
-__device__ __forceinline__ void store_codes(uint8_t* first, uint8_t* second, long long at, int left, const uint32_t (&c)[8]) {
+__device__ __forceinline__ void store_codes(uint8_t* first, uint8_t* second, long long at, int left, const uint32_t (&c1)[8],
+                                            const float (&m)[8], const uint32_t (&c2)[8]) {
   const int lane = threadIdx.x & 31;
   if (kVectors) {
-    uint32_t u[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = __byte_perm(c[2 * i], c[2 * i + 1], 0x5140);
-    *reinterpret_cast<uint2*>(first + at + 8 * lane) =
-        make_uint2(__byte_perm(u[0], u[1], 0x5410), __byte_perm(u[2], u[3], 0x5410));
-    *reinterpret_cast<uint2*>(second + at + 8 * lane) =
-        make_uint2(__byte_perm(u[0], u[1], 0x7632), __byte_perm(u[2], u[3], 0x7632));
+    *reinterpret_cast<uint2*>(first + at + 8 * lane) = make_uint2(pack_codes(c1, m), pack_codes(c1 + 4, m + 4));
+    *reinterpret_cast<uint2*>(second + at + 8 * lane) = make_uint2(pack_codes(c2), pack_codes(c2 + 4));
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int j = lane + 32 * i;
-      if (j < left) first[at + j] = (uint8_t)c[i], second[at + j] = (uint8_t)(c[i] >> 8);
+      if (j >= left) continue;
+      first[at + j] = (uint8_t)((c1[i] & 0x7Fu) | (__float_as_uint(m[i]) >> 24 & 0x80u));
+      second[at + j] = (uint8_t)c2[i];
     }
   }
 }
@@ -188,14 +196,17 @@ __device__ __forceinline__ void store_codes(uint8_t* first, uint8_t* second, lon
 __device__ __forceinline__ float uniform_low(uint32_t h) { return __uint_as_float(__byte_perm(h, 0x43000000u, 0x7610)) - 128.f; }
 __device__ __forceinline__ float uniform_high(uint32_t h) { return __uint_as_float(__byte_perm(h, 0x43000000u, 0x7632)) - 128.f; }
 
-// The e4m3 code of size >= 0 without its sign: size is cut to a multiple of its binade's step (at least the
-// subnormals' 2^-9) after `uniform` in [0, 1) steps were added.  The steps n, at most 16, are the last places of the
-// sum rounded down at 2^23; with 8 codes to a binade the code is 8 (binade - lowest) + n.
-__device__ __forceinline__ uint32_t round8(float size, float uniform) {
+// The e4m3 code of size >= 0 without its sign, in the lowest byte: size is cut to a multiple of its binade's step (at
+// least the subnormals' 2^-9) after `uniform` in [0, 1) steps were added, and is at least `least` steps.  The steps n, at
+// most 16, are the last places of the sum rounded down at 2^23; with 8 codes to a binade the code is 8 (binade -
+// lowest) + n, and the lowest binade's 8 * 121 is 256 * 4 less the 56 that the sum gets besides.  The largest size,
+// 448 (1 + 2^-22) = 14.000004 steps, and the largest uniform, 1 - 2^-16, do not reach 15.
+__device__ __forceinline__ uint32_t round8(float size, float uniform, float least) {
   const uint32_t top = max(__float_as_uint(size) & 0x7f800000u, 121u << 23);
-  const float steps = fmaf(size, __uint_as_float((257u << 23) - top), uniform);
-  const uint32_t n = __float_as_uint(__fadd_rd(steps, 8388608.f));
-  return min((top >> 20) + n - (0x4B000000u + 121 * 8), 0x7Eu);
+  const float steps = fmaxf(fmaf(size, __uint_as_float((257u << 23) - top), uniform), least);
+  uint32_t code;
+  asm("mad.hi.u32 %0, %1, 4096, %2;" : "=r"(code) : "r"(top), "r"(__float_as_uint(__fadd_rd(steps, 8388608.f + 56.f))));
+  return code;
 }
 
 // The largest magnitude of a block; NaN if it holds one, which so reaches all of it.
@@ -292,22 +303,23 @@ __device__ __forceinline__ void update_blocks(const Entry& e, const Common& c, c
       const bool none1 = top1 < kTiny, none2 = top2 < kTiny;
       const float to1 = none1 ? 0.f : 448.f * __frcp_rn(top1), to2 = none2 ? 0.f : 448.f * __frcp_rn(top2);
       const uint32_t key = tensor_key + (uint32_t)((unsigned long long)base >> 32) * 0x9E3779B9u;
-      uint32_t code[8];
+      uint32_t code1[8], code2[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t element = (uint32_t)base + (kVectors ? 8 * lane + i : lane + 32 * i);
         const uint32_t h = mix(element ^ key);
-        const float x = m[i] * to1, y = v[i] * to2;
-        code[i] = round8(fabsf(x), uniform_low(h)) | (__float_as_uint(x) >> 24 & 0x80u);
-        code[i] |= max(round8(y, uniform_high(h)), y > 0.f ? 1u : 0u) << 8;
+        const float y = v[i] * to2;
+        code1[i] = round8(fabsf(m[i] * to1), uniform_low(h), 0.f);
+        code2[i] = round8(y, uniform_high(h), fminf(y * 0x1p+126f, 1.f));  // what is not zero has a step at least
       }
       if (!(top1 <= FLT_MAX && top2 <= FLT_MAX)) {  // NaN where a scaled value is none, zero elsewhere
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          code[i] = (isnan(m[i] * to1) ? 0x7Fu : top1 <= FLT_MAX ? code[i] & 0xFFu : 0u) |
-                    (isnan(v[i] * to2) ? 0x7F00u : top2 <= FLT_MAX ? code[i] & 0xFF00u : 0u);
+        for (int i = 0; i < 8; ++i) {
+          code1[i] = isnan(m[i] * to1) ? 0x7Fu : top1 <= FLT_MAX ? code1[i] : 0u;
+          code2[i] = isnan(v[i] * to2) ? 0x7Fu : top2 <= FLT_MAX ? code2[i] : 0u;
+        }
       }
-      store_codes<kVectors>(static_cast<uint8_t*>(moment1), static_cast<uint8_t*>(moment2), base, left, code);
+      store_codes<kVectors>(static_cast<uint8_t*>(moment1), static_cast<uint8_t*>(moment2), base, left, code1, m, code2);
       if (lane == 0) {
         scale1[block] = none1 ? 0.f : top1 * (1.f / 448);
         scale2[block] = none2 ? 0.f : top2 * (1.f / 448);

@@ -799,6 +799,7 @@ int resident_clusters(const void* kernel, int cluster, size_t smem) {
     cudaLaunchAttribute attrs[2]{};
     const cudaLaunchConfig_t config = config_of(one, cluster, smem, nullptr, attrs);
     int n = 0;
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);  // clusters of more than 8 blocks
     if (cudaOccupancyMaxActiveClusters(&n, kernel, &config) != cudaSuccess) cudaGetLastError(), n = 0;
     k->clusters[cluster] = n > 0 ? n : -1;
   }
@@ -806,20 +807,19 @@ int resident_clusters(const void* kernel, int cluster, size_t smem) {
 }
 
 // The widest cluster of which the GPU holds as many at once as there are: a second wave of them would double the time
-// (16 clusters of 16 blocks: 14 are held, and 131072 x 1024 took 1214 us; of NN blocks NNN us).  A block has at least
-// one round of rows.
+// (16 clusters of 16 blocks, of which 14 are held, for 131072 x 1024: 1214 us where those of 13 took 690).  Narrower
+// ones are slower, a round takes as long with fewer rows (of 8, 9 and 11 blocks: 725, 650 and 571 us where those of 13
+// took 489).  A block has at least one round of rows.
 template <typename K>
 cudaError_t launch_divided(K kernel, RecArgs a, const Division& s, int tile_rows, size_t smem, int* parts, cudaStream_t stream) {
   const void* const pointer = reinterpret_cast<const void*>(kernel);
   cudaError_t e = ensure_dynamic_smem(pointer, (int)smem);
   const long long groups = (long long)s.tiles * s.segments, tiles = (s.rows + tile_rows - 1) / tile_rows;
   a.cluster = 1;
-  if (e == cudaSuccess && tiles > 1 && groups < 2ll * sm_count()) {
-    e = cudaFuncSetAttribute(pointer, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
+  if (tiles > 1 && groups < 2ll * sm_count())
     for (int c = (int)(tiles < kMostCluster ? tiles : kMostCluster); c > 1 && a.cluster == 1; --c)
       if (resident_clusters(pointer, c, smem) >= groups) a.cluster = c;
-  }
-  if (e != cudaSuccess) return e;
   if (parts) *parts = s.segments * a.cluster;
   cudaLaunchAttribute attrs[2]{};
   const cudaLaunchConfig_t config = config_of(s, a.cluster, smem, stream, attrs);

@@ -48,6 +48,9 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
+
+
 def _stream(device) -> int:
     """The current stream of a device as the integer the C ABI takes."""
     return _raw_stream(_device_index(device))

@@ -16,7 +16,7 @@ import math
 import torch
 
 from . import capi
-from .module import _device_index, _ptr, _stream
+from .module import _capturing, _device_index, _ptr, _stream
 from .residual_norm import _row_stride
 
 
@@ -42,6 +42,10 @@ class GatedLinearRecurrence:
         self.output = self.state = self.gradInput = self.gradProjection = self.gradState = self.checkpoints = None
         self._key = None
         self._step_key = None
+        # whether a captured graph uses the tensors that are kept for the present shapes, and such tensors of earlier
+        # shapes: a graph may be replayed after other shapes have run
+        self._captured = self._step_captured = False
+        self._graphs = []
 
     # -- nn.Module surface -------------------------------------------------------
     def training(self):
@@ -63,6 +67,8 @@ class GatedLinearRecurrence:
         x, g, z = self._prepare(input, offsets)
         self._check_state(state, "initial state")
         if state is not None and state.data_ptr() == self._state.data_ptr():
+            if self._captured:
+                self._graphs.append(self._state)
             self._state = torch.empty_like(self._state)  # what was returned before is an input now
         checkpoints = None
         if self.train:
@@ -82,12 +88,17 @@ class GatedLinearRecurrence:
     def step(self, input, state):
         """One token: x, g and z are (sequences, channels), the states are updated in place."""
         x, g, z = self._table(input)
-        key = (x.shape, x.stride(), g.stride(), None if z is None else z.stride(), x.dtype, x.device)
-        if key != self._step_key:
+        key = (x.shape, x.stride(), g.stride(), None if z is None else z.stride(), x.dtype, x.device, id(self.bias))
+        if key == self._step_key:
+            self._step_captured = self._step_captured or _capturing()
+        else:
             assert x.dim() == 2, "a step takes (sequences, channels)"
             self._check_table(x, g, z)
             self._step_desc = self._new_desc(x, g, z, None, x.shape[0], 1)
             self._step_ref = ctypes.byref(self._step_desc)
+            if self._step_captured:
+                self._graphs.append(self._step_output)
+            self._step_captured = _capturing()
             self._step_output = torch.empty(x.shape, dtype=x.dtype, device=x.device)
             self._step_key = key
         assert g.shape == x.shape and g.dtype == x.dtype and (z is None or (z.shape == x.shape and z.dtype == x.dtype))
@@ -135,7 +146,10 @@ class GatedLinearRecurrence:
         """Checks the table; descriptor and outputs are kept for one set of shapes."""
         x, g, z = self._table(input)
         key = tuple((t.shape, t.stride(), t.dtype, t.device) if t is not None else None for t in (x, g, z, offsets))
-        if key != self._key:
+        key += (id(self.bias),)
+        if key == self._key:
+            self._captured = self._captured or _capturing()
+        else:
             self._check_table(x, g, z)
             if offsets is None:
                 assert x.dim() == 3, "(batch, length, channels), or packed (rows, channels) with offsets"
@@ -148,6 +162,10 @@ class GatedLinearRecurrence:
             self._desc = self._new_desc(x, g, z, offsets, sequences, length)
             self._desc_ref = ctypes.byref(self._desc)
             self._where = x.device
+            if self._captured:
+                self._graphs.append((self._output, self._state, self._checkpoints, self._grads, self._workspace, self._grad_state))
+            self._captured = _capturing()
+            self._workspace = self._grad_state = None
             self._output = torch.empty(x.shape, dtype=x.dtype, device=x.device)
             self._state = torch.empty((sequences, self.channels), dtype=torch.float32, device=x.device)
             self._checkpoints = self._grads = None
@@ -182,6 +200,8 @@ class GatedLinearRecurrence:
         self._desc.grad_y_stride = _row_stride(gradOutput)
         states = inputs and (state is not None or gradState is not None)
         if states and gradState is not None and gradState.data_ptr() == self._grad_state.data_ptr():
+            if self._captured:
+                self._graphs.append(self._grad_state)
             self._grad_state = torch.empty_like(self._grad_state)
         grads = [_ptr(t) if inputs else None for t in self._grads] + [None] * (3 - parts)
         with_bias = parameters and self.gradBias is not None

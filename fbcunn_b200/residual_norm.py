@@ -17,7 +17,7 @@ import math
 import torch
 
 from . import capi
-from .module import _device_index, _ptr, _stream
+from .module import _capturing, _device_index, _ptr, _stream
 
 _NORMS = {None: capi.NORM_NONE, "rms": capi.NORM_RMS, "layer": capi.NORM_LAYER}
 _GATES = {None: capi.GATE_NONE, "linear": capi.GATE_LINEAR, "sigmoid": capi.GATE_SIGMOID}
@@ -60,6 +60,8 @@ class GatedResidualNorm:
         self.stats = None
         self._key = None
         self._workspace = None
+        self._captured = False  # whether a captured graph uses the tensors that are kept for the present shapes
+        self._graphs = []       # such tensors of earlier shapes: a graph may be replayed after other shapes have run
 
     # -- nn.Module surface -------------------------------------------------------
     def training(self):
@@ -118,8 +120,10 @@ class GatedResidualNorm:
         """Checks the table; descriptor and outputs are kept for one set of shapes."""
         u, r, gate = self._table(input)
         key = tuple((t.shape, t.stride(), t.dtype, t.device) if t is not None else None for t in (u, r, gate))
-        key += (self.residualScale, self.branchScale, self.eps)
+        key += (self.residualScale, self.branchScale, self.eps, id(self.postWeight), id(self.postBias), id(self.preWeight),
+                id(self.preBias))
         if key == self._key:
+            self._captured = self._captured or _capturing()
             return u, r, gate
         for t in (u, r, gate):
             if t is None:
@@ -146,6 +150,9 @@ class GatedResidualNorm:
             self.branchScale, _device_index(r.device))
         self._desc_ref = ctypes.byref(self._desc)
         self._where = r.device
+        if self._captured:
+            self._graphs.append((self._r_out, self._v, self._stats, self._grads, self._workspace))
+        self._captured = _capturing()
         self._r_out = torch.empty(r.shape, dtype=r.dtype, device=r.device) if u is not None else None
         self._v = torch.empty(r.shape, dtype=kind, device=r.device) if self.pre is not None else None
         self._stats = torch.empty((rows, 4), dtype=torch.float32, device=r.device)

@@ -330,3 +330,28 @@ def test_refusals_on_the_device():
     assert capi.lib().fbfftconv_adamw_set_gradients(opt._handle, host, 1) == capi.ERR_INVALID_ARGUMENT
     opt.step()  # the handle still has its own gradients
     assert opt.steps == 1
+
+
+def test_a_captured_step_of_many_tensors():
+    """The large table of a launch's parameters in a graph, and two such graphs of two optimizers side by side."""
+    made = []
+    for seed in (0, 1):
+        params, grads, _ = _tensors([(37 * i) % 900 + 1 for i in range(150)], torch.bfloat16, torch.float32, seed=seed)
+        twin = [p.clone() for p in params]
+        opts = [AdamW(p, grads, stateBits=8, min8bitSize=256, masters=True, **HYPER) for p in (params, twin)]
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+            opts[0].step()
+        made.append((graph, side, opts))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for graph, side, opts in made:
+            with torch.cuda.stream(side):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, (a, b) in made:
+        for _ in range(3):
+            b.step()
+        assert a.steps == b.steps == 3
+        assert all(torch.equal(p, q) for p, q in zip(a.params + a.masters, b.params + b.masters))

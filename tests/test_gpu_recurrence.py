@@ -375,3 +375,47 @@ def test_a_wait_that_nothing_ends_gives_up():
     m, table, dy, h0, dlast = make((1, 3000), 1, 64, BF, seed=7)
     check(m, table, dy, h0, dlast)
     assert lib.fbfftconv_recurrence_status(0) == 0
+
+
+def test_graphs_of_several_shapes():
+    """A graph captured for one batch is replayed after other batches have run through the module, as a server with one
+    graph for each batch size does it: nothing else may have taken the memory that the graph writes."""
+    m = GatedLinearRecurrence(64)
+    m.bias.normal_()
+    made, graphs = {}, {}
+    for n in (2, 5, 9):
+        x = [torch.randn(n, 64, device="cuda") for _ in range(3)]
+        long = [torch.randn(n, 20, 64, device="cuda") for _ in range(3)]
+        state, dy = torch.randn(n, 64, device="cuda"), torch.randn(n, 20, 64, device="cuda")
+
+        def work(x=x, long=long, state=state, dy=dy):
+            y = m.step(x, state)
+            return [y, m.updateOutput(long), *m.backward(long, dy), m.gradBias]
+
+        work()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graphs[n] = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side), torch.cuda.graph(graphs[n], stream=side):
+            made[n] = (work(), state, work)
+        torch.cuda.synchronize()
+    fill = [torch.full((n, 20, 64), 7.0, device="cuda") for n in range(1, 40)]  # what freed memory would be given to
+    for n, (outputs, state, work) in made.items():
+        start = state.clone()
+        graphs[n].replay()
+        got = [t.clone() for t in outputs]
+        state.copy_(start)
+        m.gradBias.zero_()
+        for a, b in zip(got, work()):
+            assert torch.equal(a, b)
+    assert all((t == 7).all() for t in fill)
+
+
+def test_a_replaced_bias_is_looked_at():
+    m, table, *_ = make((1, 4), 1, 32)
+    m.updateOutput(table)
+    m.bias = torch.zeros(16, device="cuda")
+    with pytest.raises(AssertionError):
+        m.updateOutput(table)
+    with pytest.raises(AssertionError):
+        m.step([t[:, 0] for t in table], torch.zeros(1, 32, device="cuda"))

@@ -303,3 +303,38 @@ def test_refusals():
                                             m.output[0].data_ptr(), host.data_ptr(), None, None]
     assert lib.fbfftconv_residual_norm(m._desc_ref, *args) == capi.ERR_INVALID_ARGUMENT
     assert "norm's output" in capi.last_error() and capi.kernel_launches() == launches
+
+
+def test_graphs_of_several_shapes():
+    """A graph captured for one batch is replayed after other batches have run through the module."""
+    m = GatedResidualNorm(96, gate="sigmoid")
+    made = {}
+    for n in (3, 8):
+        table = [torch.randn(n, 5, 96, device="cuda") for _ in range(3)]
+        grads = [torch.randn(n, 5, 96, device="cuda") for _ in range(2)]
+
+        def work(table=table, grads=grads):
+            return [*m.updateOutput(table), *m.backward(table, grads), *m.parameters()[1]]
+
+        work()
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+            outputs = work()
+        torch.cuda.synchronize()
+        made[n] = graph, outputs, work
+    fill = [torch.full((n, 5, 96), 7.0, device="cuda") for n in range(1, 40)]
+    for graph, outputs, work in made.values():
+        graph.replay()
+        got = [t.clone() for t in outputs]
+        for a, b in zip(got, work()):
+            assert torch.equal(a, b)
+    assert all((t == 7).all() for t in fill)
+
+
+def test_a_replaced_weight_is_looked_at():
+    m, table, _ = build((2, 3), 64)
+    m.updateOutput(table)
+    m.preWeight = torch.ones(32, device="cuda")
+    with pytest.raises(AssertionError):
+        m.updateOutput(table)

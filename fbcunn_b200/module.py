@@ -51,6 +51,11 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
 
 
+def _layout(t: Optional[torch.Tensor]):
+    """What a module's descriptor takes from a tensor besides its address."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
 def _stream(device) -> int:
     """The current stream of a device as the integer the C ABI takes."""
     return _raw_stream(_device_index(device))

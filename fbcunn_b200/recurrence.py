@@ -16,7 +16,7 @@ import math
 import torch
 
 from . import capi
-from .module import _capturing, _device_index, _ptr, _stream
+from .module import _capturing, _device_index, _layout, _ptr, _raw_stream, _stream
 from .residual_norm import _row_stride
 
 
@@ -88,24 +88,26 @@ class GatedLinearRecurrence:
     def step(self, input, state):
         """One token: x, g and z are (sequences, channels), the states are updated in place."""
         x, g, z = self._table(input)
-        key = (x.shape, x.stride(), g.stride(), None if z is None else z.stride(), x.dtype, x.device, id(self.bias))
-        if key == self._step_key:
-            self._step_captured = self._step_captured or _capturing()
-        else:
+        key = (_layout(x), _layout(g), _layout(z), id(self.bias))
+        if key != self._step_key:
             assert x.dim() == 2, "a step takes (sequences, channels)"
             self._check_table(x, g, z)
             self._step_desc = self._new_desc(x, g, z, None, x.shape[0], 1)
             self._step_ref = ctypes.byref(self._step_desc)
             if self._step_captured:
                 self._graphs.append(self._step_output)
-            self._step_captured = _capturing()
+            self._step_captured = False
             self._step_output = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            self._step_index, self._step_call = _device_index(x.device), capi.lib().fbfftconv_recurrence_step
             self._step_key = key
-        assert g.shape == x.shape and g.dtype == x.dtype and (z is None or (z.shape == x.shape and z.dtype == x.dtype))
+        if not self._step_captured:
+            self._step_captured = _capturing()
         assert state.shape == x.shape and state.dtype == torch.float32 and state.is_contiguous() and state.is_cuda
-        capi.check(capi.lib().fbfftconv_recurrence_step(
+        status = self._step_call(
             self._step_ref, x.data_ptr(), g.data_ptr(), _ptr(z), _ptr(self.bias), state.data_ptr(),
-            self._step_output.data_ptr(), _stream(x.device)))
+            self._step_output.data_ptr(), _raw_stream(self._step_index))
+        if status:
+            capi.check(status)
         return self._step_output
 
     def backward(self, input, gradOutput, scale=None, *, state=None, offsets=None, gradState=None):
@@ -145,10 +147,10 @@ class GatedLinearRecurrence:
     def _prepare(self, input, offsets):
         """Checks the table; descriptor and outputs are kept for one set of shapes."""
         x, g, z = self._table(input)
-        key = tuple((t.shape, t.stride(), t.dtype, t.device) if t is not None else None for t in (x, g, z, offsets))
-        key += (id(self.bias),)
+        key = (_layout(x), _layout(g), _layout(z), _layout(offsets), id(self.bias))
         if key == self._key:
-            self._captured = self._captured or _capturing()
+            if not self._captured:
+                self._captured = _capturing()
         else:
             self._check_table(x, g, z)
             if offsets is None:

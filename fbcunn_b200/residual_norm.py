@@ -17,7 +17,7 @@ import math
 import torch
 
 from . import capi
-from .module import _capturing, _device_index, _ptr, _stream
+from .module import _capturing, _device_index, _layout, _ptr, _raw_stream, _stream
 
 _NORMS = {None: capi.NORM_NONE, "rms": capi.NORM_RMS, "layer": capi.NORM_LAYER}
 _GATES = {None: capi.GATE_NONE, "linear": capi.GATE_LINEAR, "sigmoid": capi.GATE_SIGMOID}
@@ -84,9 +84,11 @@ class GatedResidualNorm:
         r_out, v = self._r_out, self._v
         stats = self._stats if self.train else None
         self.stats = stats
-        capi.check(capi.lib().fbfftconv_residual_norm(
+        status = self._forward(
             self._desc_ref, _ptr(u), r.data_ptr(), _ptr(gate), _ptr(self.postWeight), _ptr(self.postBias),
-            _ptr(self.preWeight), _ptr(self.preBias), _ptr(r_out), _ptr(v), _ptr(stats), _stream(self._where)))
+            _ptr(self.preWeight), _ptr(self.preBias), _ptr(r_out), _ptr(v), _ptr(stats), _raw_stream(self._index))
+        if status:
+            capi.check(status)
         self.output = v if u is None else r_out if v is None else [r_out, v]
         return self.output
 
@@ -119,11 +121,11 @@ class GatedResidualNorm:
     def _prepare(self, input):
         """Checks the table; descriptor and outputs are kept for one set of shapes."""
         u, r, gate = self._table(input)
-        key = tuple((t.shape, t.stride(), t.dtype, t.device) if t is not None else None for t in (u, r, gate))
-        key += (self.residualScale, self.branchScale, self.eps, id(self.postWeight), id(self.postBias), id(self.preWeight),
-                id(self.preBias))
+        key = (_layout(u), _layout(r), _layout(gate), self.residualScale, self.branchScale, self.eps, id(self.postWeight),
+               id(self.postBias), id(self.preWeight), id(self.preBias))
         if key == self._key:
-            self._captured = self._captured or _capturing()
+            if not self._captured:
+                self._captured = _capturing()
             return u, r, gate
         for t in (u, r, gate):
             if t is None:
@@ -149,7 +151,7 @@ class GatedResidualNorm:
             types[r.dtype], _NORMS[self.post], _NORMS[self.pre], _GATES[self.gate], self.eps, self.residualScale,
             self.branchScale, _device_index(r.device))
         self._desc_ref = ctypes.byref(self._desc)
-        self._where = r.device
+        self._where, self._index, self._forward = r.device, _device_index(r.device), capi.lib().fbfftconv_residual_norm
         if self._captured:
             self._graphs.append((self._r_out, self._v, self._stats, self._grads, self._workspace))
         self._captured = _capturing()

@@ -68,7 +68,7 @@ struct Common {
 };
 
 // 4 KB of parameters reach every device; larger tables take the extended limit.
-constexpr int kFew = 44, kMany = 400;
+constexpr int kFew = 44, kSome = 128, kMany = 400;
 template <int N> struct Table {
   Common c;
   Entry entry[N];
@@ -543,7 +543,9 @@ int step(fbfftconv_adamw* h, double lr, float grad_scale, const float* scalars, 
     const long long more = i < total ? blocks_of(h->tensors[i].count) : 0;
     if (i == total || n == kMany || blocks + more > kMostBlocks) {
       c.advance = i == total;
-      const cudaError_t e = n <= kFew ? launch<kFew>(h, chosen, n, c, stream) : launch<kMany>(h, chosen, n, c, stream);
+      const cudaError_t e = n <= kFew    ? launch<kFew>(h, chosen, n, c, stream)
+                            : n <= kSome ? launch<kSome>(h, chosen, n, c, stream)
+                                         : launch<kMany>(h, chosen, n, c, stream);
       if (e != cudaSuccess) return op_cuda_fail(e, "adamw");
       n = 0, blocks = 0;
     }

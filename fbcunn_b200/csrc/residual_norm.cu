@@ -411,8 +411,10 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(const NormArgs 
     int row = s * stretch + worker % splits;
     if (kRing)
       for (int k = 0; k < a.stages; ++k) fetch(row + k * splits, end, shared_gate ? s : row + k * splits, stage + k < a.stages ? stage + k : 0);
+    float4 next_stat = row < end ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
     for (; row < end; row += splits, stage = stage + 1 < a.stages ? stage + 1 : 0) {
-      const float4 stat = a.stats[row];
+      const float4 stat = next_stat;
+      if (row + splits < end) next_stat = a.stats[row + splits];  // a row ahead: nothing of a row can begin without it
       if (kRing) ring.wait();
       float x[C], d[C], w[C], act[C];  // x: the block's output, normalised
       if (need_u) {

@@ -154,6 +154,24 @@ def test_packed(lengths, dtype, wide):
         assert (t[:4] == mark).all() and (t[-6:] == mark).all()
 
 
+def test_more_sequences_than_are_kept_on_the_chip():
+    """The search goes to memory for more than 512 sequences."""
+    lengths = [(7 * i) % 5 for i in range(700)]
+    offsets = torch.tensor([0] + lengths).cumsum(0).to("cuda", torch.int32)
+    check(*make((int(offsets[-1]),), 700, 48, BF), offsets=offsets)
+
+
+def test_one_of_the_two_states():
+    m, table, dy, h0, dlast = make((2, 90), 2, 32, F32)
+    check(m, table, dy, h0, None)
+    m.updateOutput(table)
+    grads = [g.clone() for g in m.backward(table, dy, gradState=dlast)]
+    want = reference(*[t.reshape(-1, 32) for t in table], m.bias, [0, 90, 180], torch.zeros_like(h0), dy.reshape(-1, 32), dlast)
+    for k, t in zip(("dx", "dg", "dz"), grads):
+        _near(t.reshape(-1, 32).cpu(), *want[k], k)
+    _near(m.gradState.cpu(), *want["dstate"], "dstate")
+
+
 def test_channels_off_their_pairs():
     check(*make((2, 100), 2, 66, BF, shift=1))
     check(*make((3, 50), 3, 31, HF, shift=3))

@@ -298,6 +298,11 @@ struct Words {
           if (i < rows)
             asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + i * 128 + lane * 4), "l"(from + i * stride) : "memory");
       }
+    } else {
+      // to the L1 cache: a row's 32 values lie in one or two lines, and two lanes see to each row
+      const int lane = threadIdx.x & 31, row = lane >> 1;
+      if (row < kRows && row < n)
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(p + row * stride + (lane & 1 ? min(31, channels - 1 - channel) : 0)));
     }
   }
   __device__ __forceinline__ void commit() const {

@@ -7,8 +7,9 @@
 //   du = s1 (dn w1 - hat1 mean(dn w1 hat1) [- mean(dn w1)]),  dact = beta D n
 //   dw2 = sum dv hat2, db2 = sum dv, dw1 = sum dn hat1, db1 = sum dn;  dg summed over the rows that share a gate row
 //
-// A row is held in the registers of one warp or one block between its sums, so each tensor moves once and HBM bounds
-// both directions.  Sums over a row go by shuffles and one exchange through shared memory; a layer norm's deviation is
+// A row is held in the registers of one warp or one block between its sums, so each tensor moves once; 16384 x 4096 bf16
+// with a gate per token takes 424 us both ways where its bytes would take 266, bound by the latency of a row's sums and
+// by issue (43 and 92 instructions an element).  Sums over a row go by shuffles and one exchange through shared memory; a layer norm's deviation is
 // taken about the mean, in a sum of its own.  Sums over rows stay in registers while a block walks its rows, and a
 // second kernel adds the blocks' sums in a fixed order: the same call gives the same bits.
 #include <math.h>
@@ -185,6 +186,13 @@ struct Ring {
   }
 };
 
+// Without the ring: a row's lines on their way to the L1 cache while the row before it is computed.
+template <typename T, int C, int kVec, bool kRing>
+__device__ __forceinline__ void prefetch_row(const T* row, const Columns<C, kVec, kRing>& c) {
+  constexpr int kLine = 128 / (int)sizeof(T);
+  for (int i = c.lane * kLine; i < c.channels; i += c.lanes * kLine) asm volatile("prefetch.global.L1 [%0];" ::"l"(row + i));
+}
+
 // The sum of a thread's columns of a row: what lies in vectors that are not the row's stays out, whatever it holds.
 template <int C, int kVec, bool kRing, typename F>
 __device__ __forceinline__ float sum_of(const Columns<C, kVec, kRing>& c, F term) {
@@ -307,6 +315,11 @@ __global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 3 : kThreads <= 32
     } else {
       if (a.u) load_row(row_of<const T>(a.u, row, a.u_stride), c, x);
       load_row(row_of<const TR>(a.r, row, a.r_stride), c, r);
+      if (row + stride < a.rows) {
+        if (a.u) prefetch_row(row_of<const T>(a.u, row + stride, a.u_stride), c);
+        prefetch_row(row_of<const TR>(a.r, row + stride, a.r_stride), c);
+        if (a.u && a.gate_kind) prefetch_row(row_of<const T>(a.gate, gate_row_of(row + stride), a.gate_stride), c);
+      }
     }
     float2 first = make_float2(0.f, 1.f), second = first;
     if (a.u) {
@@ -414,7 +427,19 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(const NormArgs 
     float4 next_stat = row < end ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
     for (; row < end; row += splits, stage = stage + 1 < a.stages ? stage + 1 : 0) {
       const float4 stat = next_stat;
-      if (row + splits < end) next_stat = a.stats[row + splits];  // a row ahead: nothing of a row can begin without it
+      if (row + splits < end) {
+        next_stat = a.stats[row + splits];  // a row ahead: nothing of a row can begin without it
+        if (!kRing) {
+          const int next = row + splits;
+          if (need_u) prefetch_row(row_of<const T>(a.u, next, a.u_stride), c);
+          if (a.gate_kind && !shared_gate) prefetch_row(row_of<const T>(a.gate, next, a.gate_stride), c);
+          if (a.dr_out) prefetch_row(row_of<const TR>(a.dr_out, next, a.channels), c);
+          if (a.pre) {
+            prefetch_row(row_of<const TR>(a.r, next, a.r_stride), c);
+            prefetch_row(row_of<const T>(a.dv, next, a.channels), c);
+          }
+        }
+      }
       if (kRing) ring.wait();
       float x[C], d[C], w[C], act[C];  // x: the block's output, normalised
       if (need_u) {
@@ -602,18 +627,23 @@ struct Shape {
 };
 
 // Short rows share a block, a warp each; a longer row has a block to itself, whose lanes meet at its barriers.  Rows of
-// whole vectors go through the ring, as long as a thread's share of the widest fits its registers.
+// whole vectors go through the ring (8192 x 7000 f16 with a gate: 152 and 347 us forward and backward; 7001 without:
+// 483 and 1109) where one row of every tensor fits shared memory.  Sixteen columns a thread are more than the registers
+// hold with the sums over rows: eight, until a row is wider than 512 threads (4096: 663 us both ways against 675).
 Shape shape_of(int channels, int columns, bool ring) {
   const int lanes = (channels + 32 * columns - 1) / (32 * columns) * 32;
   return {lanes, lanes == 32 ? 128 : lanes, columns, ring};
 }
-Shape forward_shape(int channels, bool vectors) {
-  if (vectors && channels <= 8192) return shape_of(channels, channels > 2048 ? 16 : 8, true);
+constexpr size_t kMostShared = 226 * 1024;  // of a block, less what the kernels hold besides
+
+Shape forward_shape(int channels, int type_size, int residual_size, bool vectors) {
+  if (vectors && (size_t)channels * (2 * type_size + residual_size) <= kMostShared - 16 * 1024)
+    return shape_of(channels, channels > 2048 ? 16 : 8, true);
   return shape_of(channels, channels > 8192 ? 16 : 8, false);
 }
-// `all`: sums of biases' and shared gates' gradients are held too, which leaves registers for fewer columns.
-Shape backward_shape(int channels, bool vectors, bool all) {
-  if (vectors && channels <= 8192) return shape_of(channels, channels > 4096 ? 16 : 8, true);
+Shape backward_shape(int channels, int type_size, int residual_size, bool vectors) {
+  if (vectors && (size_t)channels * (3 * type_size + 2 * residual_size) <= kMostShared - 16 * 1024)
+    return shape_of(channels, channels > 4096 ? 16 : 8, true);
   return shape_of(channels, channels > 4096 ? 16 : 8, false);
 }
 
@@ -672,8 +702,6 @@ int check_pointers(const Pointer (&all)[N], int device, int channels, int type, 
   return FBFFTCONV_OK;
 }
 
-constexpr size_t kMostShared = 226 * 1024;  // of a block, less what the kernels hold besides
-
 template <typename K>
 cudaError_t launch_rows(K kernel, NormArgs a, const Shape& s, int grid, size_t stage_bytes, cudaStream_t stream) {
   a.stages = 2 * stage_bytes <= kMostShared ? 2 : 1;
@@ -695,18 +723,21 @@ cudaError_t forward(const NormArgs& a, const Shape& s, cudaStream_t stream) {
                           : launch_rows(norm_forward_kernel<T, TR, 16, 1024, false>, a, s, grid, 0, stream);
   const size_t stage = (size_t)s.threads * s.columns * (2 * sizeof(T) + sizeof(TR));
   if (s.columns == 8) return launch_rows(norm_forward_kernel<T, TR, 8, 256, true>, a, s, grid, stage, stream);
-  return s.threads <= 320 ? launch_rows(norm_forward_kernel<T, TR, 16, 320, true>, a, s, grid, stage, stream)
-                          : launch_rows(norm_forward_kernel<T, TR, 16, 512, true>, a, s, grid, stage, stream);
+  return s.threads <= 320   ? launch_rows(norm_forward_kernel<T, TR, 16, 320, true>, a, s, grid, stage, stream)
+         : s.threads <= 512 ? launch_rows(norm_forward_kernel<T, TR, 16, 512, true>, a, s, grid, stage, stream)
+                            : launch_rows(norm_forward_kernel<T, TR, 16, 1024, true>, a, s, grid, stage, stream);
 }
 
 template <typename T, typename TR, bool kAll>
 cudaError_t backward(const NormArgs& a, const Shape& s, int grid, cudaStream_t stream) {
   if (!s.ring)
-    return s.columns == 8 ? launch_rows(norm_backward_kernel<T, TR, 8, 512, kAll, false>, a, s, grid, 0, stream)
-                          : launch_rows(norm_backward_kernel<T, TR, 16, 1024, kAll, false>, a, s, grid, 0, stream);
+    return s.columns == 8      ? launch_rows(norm_backward_kernel<T, TR, 8, 512, kAll, false>, a, s, grid, 0, stream)
+           : s.threads <= 512 ? launch_rows(norm_backward_kernel<T, TR, 16, 512, kAll, false>, a, s, grid, 0, stream)
+                              : launch_rows(norm_backward_kernel<T, TR, 16, 1024, kAll, false>, a, s, grid, 0, stream);
   const size_t stage = (size_t)s.threads * s.columns * (3 * sizeof(T) + 2 * sizeof(TR));
-  return s.columns == 8 ? launch_rows(norm_backward_kernel<T, TR, 8, 512, kAll, true>, a, s, grid, stage, stream)
-                        : launch_rows(norm_backward_kernel<T, TR, 16, 512, kAll, true>, a, s, grid, stage, stream);
+  return s.columns == 8      ? launch_rows(norm_backward_kernel<T, TR, 8, 512, kAll, true>, a, s, grid, stage, stream)
+         : s.threads <= 512 ? launch_rows(norm_backward_kernel<T, TR, 16, 512, kAll, true>, a, s, grid, stage, stream)
+                            : launch_rows(norm_backward_kernel<T, TR, 16, 1024, kAll, true>, a, s, grid, stage, stream);
 }
 
 template <typename T, typename TR>
@@ -790,7 +821,7 @@ int fbfftconv_residual_norm(const fbfftconv_norm_desc* desc, const void* u, cons
   if (!some) return FBFFTCONV_OK;
   const OnDevice on(device);
   if (on.error() != cudaSuccess) return op_cuda_fail(on.error(), "cudaSetDevice");
-  const Shape s = forward_shape(d.channels, vectors);
+  const Shape s = forward_shape(d.channels, type_bytes(d.type), type_bytes(d.residual_type), vectors);
   a.lanes = s.lanes;
   a.u = u, a.r = r, a.gate = gate, a.w1 = post_weight, a.b1 = post_bias, a.w2 = pre_weight, a.b2 = pre_bias;
   a.r_out = r_out, a.v = v, a.stats = reinterpret_cast<float4*>(stats), a.vectors = vectors;
@@ -806,9 +837,10 @@ size_t fbfftconv_residual_norm_workspace_bytes(const fbfftconv_norm_desc* desc) 
   int device;
   if (resolve_device(desc->device, &device) != FBFFTCONV_OK) return 0;
   const OnDevice on(device);
-  size_t most = 0;  // of the shapes that the pointers' alignment and the gradients asked for may lead to
-  for (int i = 0; i < 4; ++i) {
-    const size_t n = sum_floats(*desc, deal_of(*desc, backward_shape(desc->channels, i & 1, i & 2)));
+  size_t most = 0;  // of the shapes that the pointers' alignment may lead to
+  for (int i = 0; i < 2; ++i) {
+    const Shape s = backward_shape(desc->channels, type_bytes(desc->type), type_bytes(desc->residual_type), i);
+    const size_t n = sum_floats(*desc, deal_of(*desc, s));
     most = n > most ? n : most;
   }
   return most * sizeof(float);
@@ -854,7 +886,7 @@ int fbfftconv_residual_norm_backward(const fbfftconv_norm_desc* desc, const void
   float* const outs[4] = {d.post ? grad_post_weight : nullptr, d.pre ? grad_pre_weight : nullptr,
                           d.post ? grad_post_bias : nullptr, d.pre ? grad_pre_bias : nullptr};
   const bool every = shared_gate(d) || outs[2] || outs[3];
-  const Shape s = backward_shape(d.channels, vectors, every);
+  const Shape s = backward_shape(d.channels, type_bytes(d.type), type_bytes(d.residual_type), vectors);
   Deal q{};
   if (some) {
     q = deal_of(d, s);

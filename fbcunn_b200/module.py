@@ -51,6 +51,16 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
 
 
+def _used_here(index: int, made: int, tensors) -> None:
+    """Tells the allocator that tensors made on stream `made` are used on the current stream, where that is another one:
+    a module may let go of them, for other shapes, while that stream still works on them."""
+    if _raw_stream(index) != made and not _capturing():
+        stream = torch.cuda.current_stream(index)
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+
+
 def _layout(t: Optional[torch.Tensor]):
     """What a module's descriptor takes from a tensor besides its address."""
     return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())

@@ -16,7 +16,7 @@ import math
 import torch
 
 from . import capi
-from .module import _capturing, _device_index, _layout, _ptr, _raw_stream, _stream
+from .module import _capturing, _device_index, _layout, _ptr, _raw_stream, _stream, _used_here
 from .residual_norm import _row_stride
 
 
@@ -75,6 +75,7 @@ class GatedLinearRecurrence:
             if self._checkpoints is None:
                 n = int(capi.lib().fbfftconv_recurrence_checkpoint_bytes(self._desc_ref))
                 self._checkpoints = torch.empty(max(n // 4, 1), dtype=torch.float32, device=x.device)
+                self._made = self._made if _raw_stream(self._index) == self._made else -1  # of two streams: recorded on any
             checkpoints = self._checkpoints
         capi.check(capi.lib().fbfftconv_recurrence(
             self._desc_ref, x.data_ptr(), g.data_ptr(), _ptr(z), _ptr(self.bias), _ptr(state), self._output.data_ptr(),
@@ -99,9 +100,10 @@ class GatedLinearRecurrence:
             self._step_captured = False
             self._step_output = torch.empty(x.shape, dtype=x.dtype, device=x.device)
             self._step_index, self._step_call = _device_index(x.device), capi.lib().fbfftconv_recurrence_step
-            self._step_key = key
+            self._step_key, self._step_made = key, _raw_stream(self._step_index)
         if not self._step_captured:
             self._step_captured = _capturing()
+        _used_here(self._step_index, self._step_made, (self._step_output,))
         assert state.shape == x.shape and state.dtype == torch.float32 and state.is_contiguous() and state.is_cuda
         status = self._step_call(
             self._step_ref, x.data_ptr(), g.data_ptr(), _ptr(z), _ptr(self.bias), state.data_ptr(),
@@ -151,6 +153,8 @@ class GatedLinearRecurrence:
         if key == self._key:
             if not self._captured:
                 self._captured = _capturing()
+            _used_here(self._index, self._made, (self._output, self._state, self._checkpoints, self._workspace, self._grad_state,
+                                                 self._projection if self._grads else None))
         else:
             self._check_table(x, g, z)
             if offsets is None:
@@ -163,7 +167,8 @@ class GatedLinearRecurrence:
                 sequences, length = offsets.numel() - 1, 0
             self._desc = self._new_desc(x, g, z, offsets, sequences, length)
             self._desc_ref = ctypes.byref(self._desc)
-            self._where = x.device
+            self._where, self._index = x.device, _device_index(x.device)
+            self._made = _raw_stream(self._index)
             if self._captured:
                 self._graphs.append((self._output, self._state, self._checkpoints, self._grads, self._workspace, self._grad_state))
             self._captured = _capturing()
@@ -198,6 +203,7 @@ class GatedLinearRecurrence:
             n = int(capi.lib().fbfftconv_recurrence_workspace_bytes(self._desc_ref))
             self._workspace = torch.empty(max(n, 16), dtype=torch.uint8, device=x.device)
             self._grad_state = torch.empty_like(self._state)
+            self._made = self._made if _raw_stream(self._index) == self._made else -1  # of two streams: recorded on any
             self._desc.grad_x_stride = self._desc.grad_g_stride = self._desc.grad_z_stride = parts * self.channels
         self._desc.grad_y_stride = _row_stride(gradOutput)
         states = inputs and (state is not None or gradState is not None)

@@ -17,7 +17,7 @@ import math
 import torch
 
 from . import capi
-from .module import _capturing, _device_index, _layout, _ptr, _raw_stream, _stream
+from .module import _capturing, _device_index, _layout, _ptr, _raw_stream, _stream, _used_here
 
 _NORMS = {None: capi.NORM_NONE, "rms": capi.NORM_RMS, "layer": capi.NORM_LAYER}
 _GATES = {None: capi.GATE_NONE, "linear": capi.GATE_LINEAR, "sigmoid": capi.GATE_SIGMOID}
@@ -126,6 +126,7 @@ class GatedResidualNorm:
         if key == self._key:
             if not self._captured:
                 self._captured = _capturing()
+            _used_here(self._index, self._made, (self._r_out, self._v, self._stats, self._workspace, *(self._grads or ())))
             return u, r, gate
         for t in (u, r, gate):
             if t is None:
@@ -152,13 +153,14 @@ class GatedResidualNorm:
             self.branchScale, _device_index(r.device))
         self._desc_ref = ctypes.byref(self._desc)
         self._where, self._index, self._forward = r.device, _device_index(r.device), capi.lib().fbfftconv_residual_norm
+        self._made = _raw_stream(self._index)
         if self._captured:
             self._graphs.append((self._r_out, self._v, self._stats, self._grads, self._workspace))
         self._captured = _capturing()
         self._r_out = torch.empty(r.shape, dtype=r.dtype, device=r.device) if u is not None else None
         self._v = torch.empty(r.shape, dtype=kind, device=r.device) if self.pre is not None else None
         self._stats = torch.empty((rows, 4), dtype=torch.float32, device=r.device)
-        self._grads = None
+        self._grads = self._workspace = None
         self._key = key
         self.stats = None
         return u, r, gate
@@ -187,6 +189,7 @@ class GatedResidualNorm:
             self._grads = self._new_grads(u, r, gate)
             n = int(capi.lib().fbfftconv_residual_norm_workspace_bytes(self._desc_ref))
             self._workspace = torch.empty(max(n, 16), dtype=torch.uint8, device=r.device)
+            self._made = self._made if _raw_stream(self._index) == self._made else -1  # of two streams: recorded on any
         du, dr, dgate = self._new_grads(u, r, gate) if scratch else self._grads
         weights = [_ptr(g) if parameters else None for g in (self.gradPostWeight, self.gradPostBias, self.gradPreWeight,
                                                              self.gradPreBias)]

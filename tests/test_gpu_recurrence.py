@@ -437,3 +437,26 @@ def test_a_replaced_bias_is_looked_at():
         m.updateOutput(table)
     with pytest.raises(AssertionError):
         m.step([t[:, 0] for t in table], torch.zeros(1, 32, device="cuda"))
+
+
+def test_other_shapes_while_another_stream_still_works():
+    """What the module lets go of for other shapes is not given away while the stream that used it last is at work."""
+    m, table, dy, h0, dlast = make((2, 700), 2, 64, BF)
+    small = make((1, 3), 1, 64, BF)
+    m.updateOutput(table, state=h0)
+    want = [t.clone() for t in m.backward(table, dy, state=h0, gradState=dlast)] + [m.gradBias.clone()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+        m.updateOutput(table, state=h0)
+        grads = m.backward(table, dy, state=h0, gradState=dlast)
+        got = [t.clone() for t in grads] + [m.gradBias.clone()]
+    del grads
+    m.evaluate()
+    m.updateOutput(small[1])
+    m.output = m.gradInput = m.gradProjection = m.state = m.gradState = m.checkpoints = None
+    fill = [torch.full((n,), float("nan"), device="cuda") for n in (704, 1408, 2816, 22 * 64, 2 * 64, 32 * 64, 134400, 67200, 44800)
+            for _ in range(4)]
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(torch.isnan(t).all() for t in fill)

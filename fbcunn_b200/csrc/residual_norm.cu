@@ -8,7 +8,7 @@
 //   dw2 = sum dv hat2, db2 = sum dv, dw1 = sum dn hat1, db1 = sum dn;  dg summed over the rows that share a gate row
 //
 // A row is held in the registers of one warp or one block between its sums, so each tensor moves once; 16384 x 4096 bf16
-// with a gate per token takes 424 us both ways where its bytes would take 266, bound by the latency of a row's sums and
+// with a gate per token takes 421 us both ways where its bytes would take 266, bound by the latency of a row's sums and
 // by issue (43 and 92 instructions an element).  Sums over a row go by shuffles and one exchange through shared memory; a layer norm's deviation is
 // taken about the mean, in a sum of its own.  Sums over rows stay in registers while a block walks its rows, and a
 // second kernel adds the blocks' sums in a fixed order: the same call gives the same bits.
@@ -281,7 +281,7 @@ template <int C> __device__ __forceinline__ void activate(float (&y)[C], int kin
 template <typename T, int C> constexpr int pieces_of() { return C * (int)sizeof(T) / 16; }
 
 template <typename T, typename TR, int C, int kThreads, bool kRing>
-__global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 3 : kThreads <= 320 ? 2 : 1) norm_forward_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 4 : kThreads <= 320 ? 2 : 1) norm_forward_kernel(const NormArgs a) {
   constexpr int kVec = std::is_same_v<T, float> ? 4 : 8;
   constexpr int kT = pieces_of<T, C>(), kTR = pieces_of<TR, C>();
   __shared__ __align__(16) float part[2][2][32];
@@ -716,7 +716,9 @@ cudaError_t launch_rows(K kernel, NormArgs a, const Shape& s, int grid, size_t s
 template <typename T, typename TR>
 cudaError_t forward(const NormArgs& a, const Shape& s, cudaStream_t stream) {
   const long long slots = s.threads / s.lanes, need = (a.rows + slots - 1) / slots;
-  const long long most = (long long)sm_count() * 8;
+  // a thousand threads an SM, in blocks that walk several rows each (24 x 513 x 1000 f32 both ways: 125 us, with eight
+  // blocks an SM whatever their size 131; 131072 x 256 bf16 forward 61 and 71, 8192 x 5120 113 and 115)
+  const long long most = (long long)sm_count() * (s.threads >= 256 ? 4 : 1024 / s.threads);
   const int grid = (int)(need < most ? need : most);
   if (!s.ring)
     return s.columns == 8 ? launch_rows(norm_forward_kernel<T, TR, 8, 1024, false>, a, s, grid, 0, stream)

@@ -902,6 +902,7 @@ int fbfftconv_residual_norm_backward(const fbfftconv_norm_desc* desc, const void
   int groups = 0;
   if (some) {
     a.lanes = s.lanes, a.u = u, a.r = r, a.gate = gate, a.w1 = post_weight, a.b1 = post_bias, a.w2 = pre_weight;
+    if (!u) a.alpha = 1.f;  // the forward pass takes r itself there
     a.stats = reinterpret_cast<float4*>(const_cast<float*>(stats));
     a.dr_out = grad_r, a.dv = grad_v, a.du = grad_u, a.dr = grad_r_in, a.dgate = grad_gate, a.vectors = vectors;
     a.sums = sums, a.splits = q.splits;

@@ -30,7 +30,7 @@ class GatedResidualNorm:
     u, r and the gate are (..., channels); r has u's type or fp32, the others u's.  The gate has u's shape, or one that
     is shared by consecutive rows: (batch, 1, channels) for a gate of each sequence, (1, ..., channels) or (channels)
     for one of all rows.  Without post-norm and gate the table may be [r] (or r itself): v = pre(r), the entry to the
-    first block.  Without pre-norm the output is r'.  Weights are fp32; in training() mode, the default, updateOutput
+    first block, which no scale touches.  Without pre-norm the output is r'.  Weights are fp32; in training() mode, the default, updateOutput
     leaves in `stats` what backward needs besides its inputs, and backward must follow the updateOutput of the same
     inputs.  Gradients of weights are overwritten, or added to with accumulate=True."""
 

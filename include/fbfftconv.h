@@ -411,9 +411,9 @@ int fbfftconv_recurrence_wait_selftest(fbfftconv_stream stream);
  * u, r, r', v are (rows, channels); r and r' are the residual stream, of the block's element type or fp32.  v is taken
  * from the sum before it is rounded to r'.  Either norm may be absent (not both), the gate too.  The gate g has
  * gate_rows rows, a divisor of rows: consecutive rows / gate_rows rows share one (a gate for each token, sequence, or
- * for all).  u may be null when neither post-norm nor gate is there: v = pre(r), and r' is r itself, not written.
- * weights and biases are fp32 (channels); a bias may be null.  channels <= 16384, rows and strides <= 2^30.  Rows of u, r and the gate lie
- * their stride (elements; 0 = channels) apart, everything else is contiguous. */
+ * for all).  u may be null when neither post-norm nor gate is there: v = pre(r), and r' is r itself, neither scaled nor
+ * written.  Weights and biases are fp32 (channels); a bias may be null.  channels <= 16384, rows and strides <= 2^30.
+ * Rows of u, r and the gate lie their stride (elements; 0 = channels) apart, everything else is contiguous. */
 enum { FBFFTCONV_NORM_NONE = 0, FBFFTCONV_NORM_RMS = 1, FBFFTCONV_NORM_LAYER = 2 };
 enum { FBFFTCONV_GATE_NONE = 0, FBFFTCONV_GATE_LINEAR = 1, FBFFTCONV_GATE_SIGMOID = 2 };
 typedef struct fbfftconv_norm_desc {

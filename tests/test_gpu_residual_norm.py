@@ -338,3 +338,25 @@ def test_a_replaced_weight_is_looked_at():
     m.preWeight = torch.ones(32, device="cuda")
     with pytest.raises(AssertionError):
         m.updateOutput(table)
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("channels", [320, 321])
+def test_no_scale_touches_the_entry_to_the_first_block(kind, channels):
+    """v = pre(r) whatever residualScale is, and its gradients: the same bits as with a scale of one."""
+    got = []
+    for scale in (1.0, 0.9, 0.0):
+        m, table, grads = build((4, 9), channels, BF, post=None, pre=kind, normBias=True)
+        m.residualScale = scale
+        v = m.updateOutput([table[0]])
+        got.append([v, m.backward([table[0]], grads[1]), *m.parameters()[1]])
+    x = table[0].double()
+    mean, s = _stat(x, kind, m.eps)
+    gw, hat = grads[1].double() * m.preWeight.double(), (x - mean) * s
+    want = s * (gw - hat * (gw * hat).mean(-1, keepdim=True) - (gw.mean(-1, keepdim=True) if kind == "layer" else 0))
+    off = (x.abs() + x.abs().mean(-1, keepdim=True)) * s
+    size = s * (gw.abs() + off * (gw * hat).abs().mean(-1, keepdim=True) + gw.abs().mean(-1, keepdim=True)
+                + hat.abs() * (gw.abs() * off).mean(-1, keepdim=True))
+    _near(got[0][1], want, size, "dr")
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))

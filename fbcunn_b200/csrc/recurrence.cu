@@ -325,13 +325,15 @@ struct Words {
 };
 
 // Joins what the warps and blocks before one have: a block's warps through `part`, a cluster's blocks through `whole`.
-// "Before" is in the direction of the scan; `order` counts in it.  Two buffers are used in turn where nothing but the
-// next round's barrier separates a round's reads from the next one's writes.
+// "Before" is in the direction of the scan; `order` counts in it.  Each has a buffer for even and one for odd rounds: a
+// warp that is through with a round may write the next one's while others still read, and what orders those reads is the
+// barrier of the round after, which it passes before it writes the same buffer again.
+constexpr int kTurns = 2;
 template <int V>
 struct Exchange {
-  Stretch<V> part[kWarps][32];
-  Stretch<V> whole[2][kMostCluster][32];
-  uint64_t arrived[2];  // mbarriers: the cluster's stretches of a round are there
+  Stretch<V> part[kTurns][kWarps][32];
+  Stretch<V> whole[kTurns][kMostCluster][32];
+  uint64_t arrived[kTurns];  // mbarriers: the cluster's stretches of a round are there
   int gave_up;
 };
 
@@ -356,7 +358,7 @@ __device__ __forceinline__ void start_exchange(Exchange<V>& x, int blocks) {
   if (blocks == 1) return;
   if (threadIdx.x == 0) {
     x.gave_up = 0;
-    for (int h = 0; h < 2; ++h) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&x.arrived[h])) : "memory");
+    for (int h = 0; h < kTurns; ++h) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&x.arrived[h])) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   cg::this_cluster().sync();
@@ -384,8 +386,8 @@ __device__ __forceinline__ void send(uint32_t to, uint32_t barrier, int block, c
 template <int V>
 __device__ __forceinline__ Vec<V> exchange(Exchange<V>& x, uint32_t round, int order, int rank, int blocks,
                                            const Stretch<V>& mine, Vec<V>& carry) {
-  const int lane = threadIdx.x & 31, half = round & 1;
-  Stretch<V>(*const part)[32] = blocks == 1 && half ? x.whole[0] : x.part;
+  const int lane = threadIdx.x & 31, half = round % kTurns;
+  Stretch<V>(*const part)[32] = x.part[half];
   part[order][lane] = mine;
   __syncthreads();
   Stretch<V> before = nothing<V>();
@@ -403,7 +405,7 @@ __device__ __forceinline__ Vec<V> exchange(Exchange<V>& x, uint32_t round, int o
   if (threadIdx.x == 0)
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"((uint32_t)(blocks * 32 * sizeof(Stretch<V>))) : "memory");
   for (int k = order; k < blocks; k += kWarps) send(shared_address(&x.whole[half][rank][lane]), barrier, k, all);
-  if (!*reinterpret_cast<volatile int*>(&x.gave_up) && !wait_phase(barrier, round >> 1 & 1, kMostPolls)) {
+  if (!*reinterpret_cast<volatile int*>(&x.gave_up) && !wait_phase(barrier, round / kTurns & 1, kMostPolls)) {
     x.gave_up = 1;  // the other waits of this block then run out at once: its results are lost, the kernel ends
     wait_error = 1;
   }

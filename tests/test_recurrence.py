@@ -1,7 +1,9 @@
 """The recurrence's entry points refuse bad arguments before they touch a device, and its search over packed sequences
 stays in bounds and ends for whatever the offsets hold (a host's copy of the kernel's index arithmetic)."""
 import ctypes
+import os
 import random
+import re
 
 import pytest
 
@@ -93,3 +95,70 @@ def test_search_over_any_offsets():
                 ends = {offsets[i + 1] - 1 for i in range(n) if offsets[i] < offsets[i + 1]}
                 assert [first >> i & 1 for i in range(count)] == [int(row + i in starts) for i in range(count)]
                 assert [last >> i & 1 for i in range(count)] == [int(row + i in ends) for i in range(count)]
+
+
+def _turns(name):
+    """How many buffers the exchange between warps and blocks keeps of `name`: what the kernels' source says."""
+    with open(os.path.join(fb_build.CSRC, "recurrence.cu")) as f:
+        source = f.read()
+    constant = int(re.search(r"constexpr int kTurns = (\d+);", source).group(1))
+    fields = re.search(r"struct Exchange \{(.*?)\};", source, re.S).group(1)
+    return constant if re.search(r"\b%s\[kTurns\]" % name, fields) else 1
+
+
+def _unordered(blocks, backward, part, whole, warps=8, rounds=5):
+    """Reads and writes of the same place of a cluster's exchange that nothing orders, at least one of them a write:
+    barriers, the counted stores that a wait is for and each warp's program order are what orders them."""
+    before, at = [], {}  # for each event the events that it follows, as bits; places -> [(event, is a write)]
+
+    def event(*after, use=()):
+        seen = 0
+        for a in after:
+            seen |= before[a] | 1 << a
+        before.append(seen)
+        for place, write in use:
+            at.setdefault(place, []).append((len(before) - 1, write))
+        return len(before) - 1
+
+    last = {(b, w): event() for b in range(blocks) for w in range(warps)}
+    everyone = [(b, w) for b in range(blocks) for w in range(warps)]
+
+    def barrier():
+        for b in range(blocks):
+            met = event(*[last[b, w] for w in range(warps)])
+            for w in range(warps):
+                last[b, w] = event(last[b, w], met)
+
+    for r in range(rounds):
+        order = lambda w: warps - 1 - w if backward else w
+        if backward:
+            barrier()  # the one of the rows' states
+        for b, w in everyone:
+            last[b, w] = event(last[b, w], use=[(("part", b, r % part, order(w)), True)])
+        barrier()
+        for b, w in everyone:
+            last[b, w] = event(last[b, w], use=[(("part", b, r % part, k), False) for k in range(warps) if k != order(w)])
+        armed, sent = {}, {b: [] for b in range(blocks)}
+        for b in range(blocks):
+            if blocks > 1:
+                last[b, 0] = armed[b] = event(last[b, 0])
+        for b, w in everyone:
+            for k in range(order(w), blocks if blocks > 1 else 0, warps):
+                last[b, w] = event(last[b, w], use=[(("whole", k, r % whole, b), True)])
+                sent[k].append(last[b, w])
+        for b, w in everyone:
+            if blocks > 1:
+                last[b, w] = event(last[b, w], armed[b], *sent[b])
+                last[b, w] = event(last[b, w], use=[(("whole", b, r % whole, k), False) for k in range(blocks)])
+    return {place[0] for place, uses in at.items() for i, (x, wx) in enumerate(uses) for y, wy in uses[i + 1:]
+            if (wx or wy) and not (before[y] >> x & 1 or before[x] >> y & 1)}
+
+
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("blocks", [1, 2, 3, 10])
+def test_nothing_is_written_while_it_is_read(blocks, backward):
+    assert not _unordered(blocks, backward, _turns("part"), _turns("whole"))
+    # one buffer of the warps' stretches would be written early in the forward pass, one of the blocks' in both
+    assert _unordered(blocks, backward, 1, 2) == (set() if backward else {"part"})
+    if blocks > 1:
+        assert "whole" in _unordered(blocks, backward, 2, 1)

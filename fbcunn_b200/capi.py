@@ -164,6 +164,7 @@ _SIGNATURES = {
     "fbfftconv_recurrence_backward": (c_int, [c_void_p] * 14 + [c_float, c_int, c_void_p, c_size_t, c_void_p]),
     "fbfftconv_recurrence_status": (c_int, [c_int]),
     "fbfftconv_recurrence_wait_selftest": (c_int, [c_void_p]),
+    "fbfftconv_recurrence_wait_limit": (c_uint32, [c_uint32]),
     "fbfftconv_recurrence_step": (c_int, [c_void_p] * 8),
     "fbfftconv_profile_enable": (c_int, [c_void_p, c_int]),
     "fbfftconv_profile_reset": (c_int, [c_void_p]),

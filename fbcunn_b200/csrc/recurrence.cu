@@ -16,6 +16,7 @@
 #include <cooperative_groups.h>
 #include <math.h>
 
+#include <atomic>
 #include <mutex>
 #include <type_traits>
 
@@ -58,6 +59,7 @@ struct RecArgs {
   int checkpoints_per_segment;
   int channels, wide_offsets, cluster;
   bool wide;             // rows begin on 16 bytes
+  uint32_t polls;        // of a wait for a cluster's stretches
 };
 
 // Offsets of up to this many sequences are kept in shared memory: a search is a chain of loads.
@@ -339,7 +341,7 @@ struct Exchange {
 
 __device__ int wait_error;  // set when a wait for a cluster's stretches ran out
 
-constexpr uint32_t kMostPolls = 1u << 20;  // of a microsecond: about a second, where a round takes some microseconds
+constexpr uint32_t kPolls = 1u << 20;  // of a microsecond each: about a second, where a round takes some microseconds
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -381,11 +383,11 @@ __device__ __forceinline__ void send(uint32_t to, uint32_t barrier, int block, c
 // `mine`: this warp's stretch; returns the value that enters it and moves `carry` behind the whole round.  A block's
 // stretch goes to all blocks of the cluster with the bytes counted on their mbarriers: a cluster's barrier would have
 // waited for the outputs that are on their way to memory too.  A block sends a round's stretch after all of its warps
-// have read the round's before, so that nothing arrives in a buffer that is still read, and it has all that is sent to it
-// when it leaves.
+// have read the round's before, so that nothing arrives in a buffer that is still read.  A block whose wait has run out
+// goes through its rounds without sending, counting or waiting any more, so that the others' waits run out in turn.
 template <int V>
 __device__ __forceinline__ Vec<V> exchange(Exchange<V>& x, uint32_t round, int order, int rank, int blocks,
-                                           const Stretch<V>& mine, Vec<V>& carry) {
+                                           uint32_t polls, const Stretch<V>& mine, Vec<V>& carry) {
   const int lane = threadIdx.x & 31, half = round % kTurns;
   Stretch<V>(*const part)[32] = x.part[half];
   part[order][lane] = mine;
@@ -402,11 +404,12 @@ __device__ __forceinline__ Vec<V> exchange(Exchange<V>& x, uint32_t round, int o
     return enter;
   }
   const uint32_t barrier = shared_address(&x.arrived[half]);
-  if (threadIdx.x == 0)
+  const bool lost = *reinterpret_cast<volatile int*>(&x.gave_up);
+  if (threadIdx.x == 0 && !lost)
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"((uint32_t)(blocks * 32 * sizeof(Stretch<V>))) : "memory");
-  for (int k = order; k < blocks; k += kWarps) send(shared_address(&x.whole[half][rank][lane]), barrier, k, all);
-  if (!*reinterpret_cast<volatile int*>(&x.gave_up) && !wait_phase(barrier, round / kTurns & 1, kMostPolls)) {
-    x.gave_up = 1;  // the other waits of this block then run out at once: its results are lost, the kernel ends
+  for (int k = lost ? blocks : order; k < blocks; k += kWarps) send(shared_address(&x.whole[half][rank][lane]), barrier, k, all);
+  if (!lost && !wait_phase(barrier, round / kTurns & 1, polls)) {
+    *reinterpret_cast<volatile int*>(&x.gave_up) = 1;
     wait_error = 1;
   }
 #pragma unroll 4
@@ -415,6 +418,16 @@ __device__ __forceinline__ Vec<V> exchange(Exchange<V>& x, uint32_t round, int o
 #pragma unroll 4
   for (int k = rank; k < blocks; ++k) carry = apply(x.whole[half][k][lane], carry);
   return enter;
+}
+
+// Ends a block's part: nothing may arrive in the memory of a block that has left.  One whose waits have all ended has what
+// is sent to it; one whose wait ran out stays until no other block can send any more, and then for as long as what was
+// sent may be under way.
+template <int V>
+__device__ __forceinline__ void finish_exchange(Exchange<V>& x, int blocks) {
+  if (blocks == 1) return;
+  cg::this_cluster().sync();  // every block comes here: all waits before it are bounded
+  if (*reinterpret_cast<volatile int*>(&x.gave_up)) __nanosleep(1000000);
 }
 
 // Starts a wait that nothing ends, with a limit of a few polls: 1 when it gave up.
@@ -525,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const _
     if (within) scan(std::true_type{});
     else scan(std::false_type{});
     fetch_inputs(round + 1);
-    Vec<V> h = exchange(shared, (uint32_t)round, warp, rank, blocks, mine, carry);
+    Vec<V> h = exchange(shared, (uint32_t)round, warp, rank, blocks, a.polls, mine, carry);
     words.wait();
     if (a.checkpoints && n > 0 && on && (row - begin) % kCheckpoint == 0)
       store_floats(a.checkpoints + (long long)(blockIdx.y * a.checkpoints_per_segment + (row - begin) / kCheckpoint) * a.channels + c, h);
@@ -550,6 +563,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const _
     else emit(std::false_type{});
     fetch_outputs(round + 1);
   }
+  finish_exchange(shared, blocks);
 }
 
 template <typename T, int V, bool kGate>
@@ -680,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
     if (within) through(std::true_type{});
     else through(std::false_type{});
     fetch_outputs(round + 1);
-    Vec<V> d = exchange(shared, (uint32_t)round, kWarps - 1 - warp, rank, blocks, mine, carry);
+    Vec<V> d = exchange(shared, (uint32_t)round, kWarps - 1 - warp, rank, blocks, a.polls, mine, carry);
     T* dx = static_cast<T*>(a.dx) + (long long)row * a.dx_stride + c;
     T* dg = static_cast<T*>(a.dg) + (long long)row * a.dg_stride + c;
     const auto emit = [&](auto plain) {
@@ -704,6 +718,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
     if (within) emit(std::true_type{});
     else emit(std::false_type{});
   }
+  finish_exchange(shared, blocks);
   if (!a.sums) return;
   __syncthreads();
   states[0][warp][lane].H = dbias;
@@ -909,11 +924,13 @@ int check_rec_pointers(const RowPointer (&rows)[N], const RowPointer (&floats)[M
   return validate_device_pointer(device, d.offsets, "offsets");
 }
 
+std::atomic<uint32_t> wait_polls{kPolls};
+
 RecArgs common_args(const fbfftconv_recurrence_desc& d) {
   const auto or_dense = [&](int64_t s) { return s ? (int)s : d.channels; };
   RecArgs a{};
   a.rows = (int)d.rows, a.length = (int)d.length, a.sequences = (int)d.sequences, a.channels = d.channels;
-  a.offsets = d.offsets, a.wide_offsets = d.wide_offsets;
+  a.offsets = d.offsets, a.wide_offsets = d.wide_offsets, a.polls = wait_polls.load(std::memory_order_relaxed);
   a.x_stride = or_dense(d.x_stride), a.g_stride = or_dense(d.g_stride), a.z_stride = or_dense(d.z_stride);
   a.y_stride = or_dense(d.y_stride), a.dy_stride = or_dense(d.grad_y_stride);
   a.dx_stride = or_dense(d.grad_x_stride), a.dg_stride = or_dense(d.grad_g_stride), a.dz_stride = or_dense(d.grad_z_stride);
@@ -1041,6 +1058,8 @@ int fbfftconv_recurrence_status(int reset) {
   }
   return code;
 }
+
+uint32_t fbfftconv_recurrence_wait_limit(uint32_t microseconds) { return wait_polls.exchange(microseconds); }
 
 int fbfftconv_recurrence_wait_selftest(fbfftconv_stream stream) {
   int* out = nullptr;

@@ -402,6 +402,9 @@ int fbfftconv_recurrence_step(const fbfftconv_recurrence_desc* desc, const void*
  * the device.  The self-test makes such a wait run out: FBFFTCONV_OK when it gave up as designed. */
 int fbfftconv_recurrence_status(int reset);
 int fbfftconv_recurrence_wait_selftest(fbfftconv_stream stream);
+/* The limit of those waits for the calls (and captures) from now on, in microseconds, about a second at first; returns
+ * the one before.  0: a wait whose results are not there yet gives up at once. */
+uint32_t fbfftconv_recurrence_wait_limit(uint32_t microseconds);
 
 /* ---- norms before and after a residual block ------------------------------------------------
  * One call at the border between two blocks of a residual network: the norm after the block that ends, its gate, the

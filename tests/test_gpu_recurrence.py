@@ -460,3 +460,24 @@ def test_other_shapes_while_another_stream_still_works():
             for _ in range(4)]
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(torch.isnan(t).all() for t in fill)
+
+
+def test_waits_that_run_out_in_the_middle_of_a_call():
+    """With no time to wait, the blocks of a cluster go their ways, and the call ends: its results are lost, the status
+    says so, and the calls after it are as ever."""
+    lib = capi.lib()
+    made = [make((1, 3000), 1, 64, BF, seed=11), make((3000,), 2, 33, F32, seed=12)]
+    offsets = [None, torch.tensor([0, 1100, 3000], dtype=torch.int32, device="cuda")]
+    before = lib.fbfftconv_recurrence_wait_limit(0)
+    try:
+        for (m, table, dy, h0, dlast), at in zip(made, offsets):
+            for _ in range(20):
+                m.updateOutput(table, state=h0, offsets=at)
+                m.backward(table, dy, state=h0, offsets=at, gradState=dlast)
+            torch.cuda.synchronize()
+    finally:
+        lib.fbfftconv_recurrence_wait_limit(before)
+    assert lib.fbfftconv_recurrence_status(1) == 1 and lib.fbfftconv_recurrence_status(0) == 0
+    for (m, table, dy, h0, dlast), at in zip(made, offsets):
+        check(m, table, dy, h0, dlast, at)
+    assert lib.fbfftconv_recurrence_status(0) == 0

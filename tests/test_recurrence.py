@@ -162,3 +162,55 @@ def test_nothing_is_written_while_it_is_read(blocks, backward):
     assert _unordered(blocks, backward, 1, 2) == (set() if backward else {"part"})
     if blocks > 1:
         assert "whole" in _unordered(blocks, backward, 2, 1)
+
+
+def _run_cluster(rng, blocks, rounds, stays):
+    """One run of a cluster whose waits may run out, in an order of steps that chance decides: the blocks that were sent
+    to after they had left, and whether all ended.  A block waits for all stretches of a round, or until chance ends the
+    wait; after that it goes on without sending, counting or waiting."""
+    state = [dict(round=0, step="send", lost=False, got=[0] * (rounds + 2)) for _ in range(blocks)]
+    arrived, sent_to_the_gone = 0, set()
+    for _ in range(200 * blocks * rounds):
+        alive = [b for b in state if b["step"] != "gone"]
+        if not alive:
+            break
+        b = rng.choice(alive)
+        if b["step"] == "send":
+            if not b["lost"]:
+                for k, other in enumerate(state):
+                    if other["step"] == "gone":
+                        sent_to_the_gone.add(k)
+                    other["got"][b["round"]] += 1
+            b["step"] = "wait"
+        elif b["step"] == "wait":
+            if not b["lost"] and b["got"][b["round"]] < blocks:
+                if rng.random() > 0.02:
+                    continue
+                b["lost"] = True
+            b["round"] += 1
+            b["step"] = "send" if b["round"] < rounds else "end"
+            if b["step"] == "end":
+                arrived += 1
+        elif not stays or arrived == blocks:
+            b["step"] = "gone"
+    return sent_to_the_gone, all(b["step"] == "gone" for b in state)
+
+
+def test_a_block_whose_wait_ran_out_stays_until_no_other_can_send():
+    with open(os.path.join(fb_build.CSRC, "recurrence.cu")) as f:
+        kernels = [k.split("\ntemplate")[0] for k in f.read().split("__launch_bounds__(kThreads, 2)")[1:]]
+    assert len(kernels) == 2
+    stays = all(k.rfind("finish_exchange(") > k.rfind("exchange(shared, (uint32_t)round") > 0 for k in kernels)
+    rng, too_early = random.Random(3), 0
+    for trial in range(400):
+        blocks, rounds = rng.randint(2, 16), rng.randint(1, 6)
+        gone, ended = _run_cluster(rng, blocks, rounds, stays)
+        assert not gone and ended
+        too_early += bool(_run_cluster(rng, blocks, rounds, False)[0])
+    assert too_early  # what the last barrier is for
+
+
+def test_the_limit_of_waits(lib):
+    before = lib.fbfftconv_recurrence_wait_limit(5)
+    assert before >= 100000 and lib.fbfftconv_recurrence_wait_limit(before) == 5
+    assert lib.fbfftconv_recurrence_wait_limit(before) == before

@@ -15,6 +15,7 @@
 // do not drift.
 #include <cooperative_groups.h>
 #include <math.h>
+#include <string.h>
 
 #include <atomic>
 #include <mutex>
@@ -60,6 +61,7 @@ struct RecArgs {
   int channels, wide_offsets, cluster;
   bool wide;             // rows begin on 16 bytes
   uint32_t polls;        // of a wait for a cluster's stretches
+  int* wait_error;       // set when one ran out: the device's word in host memory
 };
 
 // Offsets of up to this many sequences are kept in shared memory: a search is a chain of loads.
@@ -339,8 +341,6 @@ struct Exchange {
   int gave_up;
 };
 
-__device__ int wait_error;  // set when a wait for a cluster's stretches ran out
-
 constexpr uint32_t kPolls = 1u << 20;  // of a microsecond each: about a second, where a round takes some microseconds
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -387,7 +387,7 @@ __device__ __forceinline__ void send(uint32_t to, uint32_t barrier, int block, c
 // goes through its rounds without sending, counting or waiting any more, so that the others' waits run out in turn.
 template <int V>
 __device__ __forceinline__ Vec<V> exchange(Exchange<V>& x, uint32_t round, int order, int rank, int blocks,
-                                           uint32_t polls, const Stretch<V>& mine, Vec<V>& carry) {
+                                           const RecArgs& a, const Stretch<V>& mine, Vec<V>& carry) {
   const int lane = threadIdx.x & 31, half = round % kTurns;
   Stretch<V>(*const part)[32] = x.part[half];
   part[order][lane] = mine;
@@ -408,9 +408,9 @@ __device__ __forceinline__ Vec<V> exchange(Exchange<V>& x, uint32_t round, int o
   if (threadIdx.x == 0 && !lost)
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"((uint32_t)(blocks * 32 * sizeof(Stretch<V>))) : "memory");
   for (int k = lost ? blocks : order; k < blocks; k += kWarps) send(shared_address(&x.whole[half][rank][lane]), barrier, k, all);
-  if (!lost && !wait_phase(barrier, round / kTurns & 1, polls)) {
+  if (!lost && !wait_phase(barrier, round / kTurns & 1, a.polls)) {
     *reinterpret_cast<volatile int*>(&x.gave_up) = 1;
-    wait_error = 1;
+    *reinterpret_cast<volatile int*>(a.wait_error) = 1;
   }
 #pragma unroll 4
   for (int k = 0; k < rank; ++k) carry = apply(x.whole[half][k][lane], carry);
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const _
     if (within) scan(std::true_type{});
     else scan(std::false_type{});
     fetch_inputs(round + 1);
-    Vec<V> h = exchange(shared, (uint32_t)round, warp, rank, blocks, a.polls, mine, carry);
+    Vec<V> h = exchange(shared, (uint32_t)round, warp, rank, blocks, a, mine, carry);
     words.wait();
     if (a.checkpoints && n > 0 && on && (row - begin) % kCheckpoint == 0)
       store_floats(a.checkpoints + (long long)(blockIdx.y * a.checkpoints_per_segment + (row - begin) / kCheckpoint) * a.channels + c, h);
@@ -694,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
     if (within) through(std::true_type{});
     else through(std::false_type{});
     fetch_outputs(round + 1);
-    Vec<V> d = exchange(shared, (uint32_t)round, kWarps - 1 - warp, rank, blocks, a.polls, mine, carry);
+    Vec<V> d = exchange(shared, (uint32_t)round, kWarps - 1 - warp, rank, blocks, a, mine, carry);
     T* dx = static_cast<T*>(a.dx) + (long long)row * a.dx_stride + c;
     T* dg = static_cast<T*>(a.dg) + (long long)row * a.dg_stride + c;
     const auto emit = [&](auto plain) {
@@ -926,6 +926,43 @@ int check_rec_pointers(const RowPointer (&rows)[N], const RowPointer (&floats)[M
 
 std::atomic<uint32_t> wait_polls{kPolls};
 
+// A word for each device, in host memory that its kernels write: what a call lost is known to the next one without a wait
+// for the device.  Null where there is none to be had.
+constexpr int kMostDevices = 256;
+int* wait_error_of(int device) {
+  static std::atomic<int*> known{nullptr};
+  static std::mutex lock;
+  int* words = known.load(std::memory_order_acquire);
+  if (!words) {
+    const std::lock_guard<std::mutex> hold(lock);
+    words = known.load(std::memory_order_acquire);
+    if (!words) {
+      // the first call of a process may be one that is captured, which does not concern this allocation
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      void* p = nullptr;
+      const cudaError_t e = cudaHostAlloc(&p, kMostDevices * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      if (e != cudaSuccess) {
+        cudaGetLastError();
+        return nullptr;
+      }
+      words = static_cast<int*>(p);
+      memset(words, 0, kMostDevices * sizeof(int));
+      known.store(words, std::memory_order_release);
+    }
+  }
+  return device >= 0 && device < kMostDevices ? words + device : nullptr;
+}
+
+int take_wait_error(int device, int** out) {
+  *out = wait_error_of(device);
+  if (!*out) return op_fail(FBFFTCONV_ERR_NOMEM, "no host memory for the waits' status");
+  if (*static_cast<volatile int*>(*out))
+    return op_fail(FBFFTCONV_ERR_CUDA, "a recurrence gave up a bounded wait: results since the last fbfftconv_recurrence_status(1) are incomplete");
+  return FBFFTCONV_OK;
+}
+
 RecArgs common_args(const fbfftconv_recurrence_desc& d) {
   const auto or_dense = [&](int64_t s) { return s ? (int)s : d.channels; };
   RecArgs a{};
@@ -990,6 +1027,7 @@ int fbfftconv_recurrence(const fbfftconv_recurrence_desc* desc, const void* x, c
   if (d.sequences == 0) return FBFFTCONV_OK;
   const OnDevice on(device);
   if (on.error() != cudaSuccess) return op_cuda_fail(on.error(), "cudaSetDevice");
+  OP_TRY(take_wait_error(device, &a.wait_error));
   const Division s = division_for(d, pairs);
   a.x = x, a.g = g, a.z = z, a.bias = bias, a.state0 = state0, a.y = y, a.state = state, a.checkpoints = checkpoints;
   a.per_segment = (int)s.per_segment, a.checkpoints_per_segment = (int)s.checkpoints;
@@ -1031,6 +1069,7 @@ int fbfftconv_recurrence_backward(const fbfftconv_recurrence_desc* desc, const v
     return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "the workspace is smaller than fbfftconv_recurrence_workspace_bytes");
   const cudaStream_t cuda_stream = static_cast<cudaStream_t>(stream);
   if (d.sequences > 0) {
+    OP_TRY(take_wait_error(device, &a.wait_error));
     a.x = x, a.g = g, a.z = z, a.bias = bias, a.state0 = state0, a.checkpoints = const_cast<float*>(checkpoints);
     a.dy = grad_y, a.dstate = grad_state, a.dx = grad_x, a.dg = grad_g, a.dz = grad_z, a.dstate0 = grad_state0;
     a.sums = grad_bias ? static_cast<float*>(workspace) : nullptr;
@@ -1049,13 +1088,15 @@ int fbfftconv_recurrence_backward(const fbfftconv_recurrence_desc* desc, const v
 }
 
 int fbfftconv_recurrence_status(int reset) {
-  int code = 0;
-  const int zero = 0;
-  if (cudaMemcpyFromSymbol(&code, wait_error, sizeof(code)) != cudaSuccess ||
-      (reset && code && cudaMemcpyToSymbol(wait_error, &zero, sizeof(zero)) != cudaSuccess)) {
+  int device;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceSynchronize() != cudaSuccess) {
     cudaGetLastError();
     return -1;
   }
+  volatile int* const word = wait_error_of(device);
+  if (!word) return -1;
+  const int code = *word;
+  if (reset) *word = 0;
   return code;
 }
 

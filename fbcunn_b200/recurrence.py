@@ -61,6 +61,12 @@ class GatedLinearRecurrence:
         if self.gradBias is not None:
             self.gradBias.zero_()
 
+    def status(self, reset=False):
+        """0, or 1 when blocks of a call that wait for one another gave up doing so since the last reset (waits for the
+        device): that call's results are lost, and later calls raise until the status is reset."""
+        with torch.cuda.device(self.device):
+            return int(capi.lib().fbfftconv_recurrence_status(int(reset)))
+
     def updateOutput(self, input, state=None, offsets=None):
         """state: the initial states, or None for zeros; offsets: int32 or int64, sequences + 1 on the device, for packed
         rows, of which those outside of all sequences stay as they are in `output`."""

@@ -398,8 +398,10 @@ int fbfftconv_recurrence_step(const fbfftconv_recurrence_desc* desc, const void*
                               const float* bias, float* state, void* y, fbfftconv_stream stream);
 
 /* Long sequences of few channels go over clusters of blocks that wait for one another's results; the waits are bounded.
- * 0, or 1 when one has run out since the last reset: that call's results are lost.  -1: the query failed.  Waits for
- * the device.  The self-test makes such a wait run out: FBFFTCONV_OK when it gave up as designed. */
+ * Where one runs out, that call's results are lost, and the calls that follow on the device are refused with
+ * FBFFTCONV_ERR_CUDA as soon as that is known, until the status is reset.  The status waits for the current device:
+ * 0, or 1 when a wait has run out there since the last reset; -1: the query failed.  The self-test makes such a wait
+ * run out: FBFFTCONV_OK when it gave up as designed. */
 int fbfftconv_recurrence_status(int reset);
 int fbfftconv_recurrence_wait_selftest(fbfftconv_stream stream);
 /* The limit of those waits for the calls (and captures) from now on, in microseconds, about a second at first; returns

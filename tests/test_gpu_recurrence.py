@@ -473,11 +473,44 @@ def test_waits_that_run_out_in_the_middle_of_a_call():
         for (m, table, dy, h0, dlast), at in zip(made, offsets):
             for _ in range(20):
                 m.updateOutput(table, state=h0, offsets=at)
+                assert lib.fbfftconv_recurrence_status(1) == 1
                 m.backward(table, dy, state=h0, offsets=at, gradState=dlast)
-            torch.cuda.synchronize()
+                assert lib.fbfftconv_recurrence_status(1) == 1
     finally:
         lib.fbfftconv_recurrence_wait_limit(before)
-    assert lib.fbfftconv_recurrence_status(1) == 1 and lib.fbfftconv_recurrence_status(0) == 0
+    assert lib.fbfftconv_recurrence_status(0) == 0
     for (m, table, dy, h0, dlast), at in zip(made, offsets):
         check(m, table, dy, h0, dlast, at)
     assert lib.fbfftconv_recurrence_status(0) == 0
+
+
+def test_a_lost_call_is_not_passed_over():
+    """The calls after one whose waits ran out are refused until the status is reset, on a stream of its own too, and
+    also where the first that lost its results was a replayed one."""
+    lib = capi.lib()
+    m, table, dy, h0, dlast = make((1, 3000), 1, 64, BF, seed=13)
+    m.updateOutput(table, state=h0)
+    m.backward(table, dy, state=h0)
+    before = lib.fbfftconv_recurrence_wait_limit(0)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    try:
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            m.updateOutput(table, state=h0)
+        assert m.status() == 1  # waits for the device, whatever stream the call was on
+        with pytest.raises(capi.FbfftconvError, match="gave up"):
+            m.updateOutput(table, state=h0)
+        with pytest.raises(capi.FbfftconvError, match="gave up"):
+            m.backward(table, dy, state=h0)
+        assert m.status(reset=True) == 1 and m.status() == 0
+        with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+            m.updateOutput(table, state=h0)
+    finally:
+        lib.fbfftconv_recurrence_wait_limit(before)
+    check(m, table, dy, h0, dlast)
+    graph.replay()
+    torch.cuda.synchronize()
+    with pytest.raises(capi.FbfftconvError, match="gave up"):
+        m.updateOutput(table, state=h0)
+    assert m.status(reset=True) == 1
+    check(m, table, dy, h0, dlast)

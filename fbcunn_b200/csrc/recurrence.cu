@@ -233,6 +233,9 @@ template <int V> __device__ __forceinline__ Vec<V> sigmoid(Vec<V> x) {
   return r;
 }
 
+// z sigmoid(z) by itself: with another factor the product of a mask's lowest z would be infinite before it meets its zero.
+template <int V> __device__ __forceinline__ Vec<V> silu(Vec<V> z) { return z * sigmoid(z); }
+
 template <int V> __device__ __forceinline__ Vec<V> load_floats(const float* p) {
   Vec<V> r;
 #pragma unroll
@@ -552,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const _
         Vec<V> out = h;
         if (kGate) {
           const Vec<V> z = words.read(kZ, zs, a.z_stride, i);
-          out = (h * z) * sigmoid(z);
+          out = h * silu(z);
         }
         if (on) store_word<T, V>(y + i * a.y_stride, out);
         if (!plain && (at.last >> i & 1) && a.state && on)
@@ -758,7 +761,7 @@ __global__ void __launch_bounds__(128) recurrence_step_kernel(const RecArgs a) {
     Vec<V> out = h;
     if (kGate) {
       const Vec<V> z = unpack<T, V>(load_word<T, V>(static_cast<const T*>(a.z) + s * a.z_stride + c));
-      out = (h * z) * sigmoid(z);
+      out = h * silu(z);
     }
     store_floats(state, h);
     store_word<T, V>(static_cast<T*>(a.y) + s * a.y_stride + c, out);

@@ -514,3 +514,25 @@ def test_a_lost_call_is_not_passed_over():
         m.updateOutput(table, state=h0)
     assert m.status(reset=True) == 1
     check(m, table, dy, h0, dlast)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, HF])
+def test_output_gates_that_are_masked(dtype):
+    """z at the type's lowest value is a gate of zero whatever the state is, and at its largest one that passes all on."""
+    m = GatedLinearRecurrence(16)
+    x = torch.full((1, 5, 16), 6.0, dtype=dtype, device="cuda")
+    z = torch.full_like(x, torch.finfo(dtype).min)
+    table, one = [x, torch.zeros_like(x), z], torch.ones_like(x)
+    assert not m.updateOutput(table).any() and torch.isfinite(m.state).all()
+    for grad in m.backward(table, one):
+        assert not grad.any()
+    state = torch.full((1, 16), 6.0, device="cuda")
+    assert not m.step([t[:, 0] for t in table], state).any() and (state == 6).all()
+    z.fill_(torch.finfo(dtype).max)
+    x.fill_(2.0 ** -10)
+    h = 2.0 ** -10 * (1 - 0.5 ** torch.arange(1, 6, device="cuda").double())
+    y = m.updateOutput(table)[0, :, 0].double()
+    assert ((y - h * z[0, 0, 0].double()).abs() <= torch.finfo(dtype).eps * y).all()
+    dx, dg, dz = m.backward(table, one * 2.0 ** -20)
+    assert all(torch.isfinite(g).all() for g in (dx, dg, dz))
+    assert ((dz[0, :, 0].double() - h * 2.0 ** -20).abs() <= torch.finfo(dtype).eps * h * 2.0 ** -20 + 2.0 ** -25).all()

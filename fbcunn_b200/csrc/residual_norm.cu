@@ -917,6 +917,10 @@ int fbfftconv_residual_norm_backward(const fbfftconv_norm_desc* desc, const void
 #undef BACKWARD
     if (e != cudaSuccess) return op_cuda_fail(e, "residual norm, backward");
   }
+  if (!some && d.gate && grad_gate && d.gate_rows > 0) {  // gate rows that no rows share
+    const cudaError_t e = cudaMemsetAsync(grad_gate, 0, (size_t)d.gate_rows * d.channels * type_bytes(d.type), cuda_stream);
+    if (e != cudaSuccess) return op_cuda_fail(e, "residual norm, backward");
+  }
   if (sum.jobs + groups == 0) return FBFFTCONV_OK;
   count_launch();
   const cudaError_t e = launch_dependent(norm_sum_kernel, dim3((d.channels + 31) / 32, sum.jobs + groups), 1024, 0, cuda_stream, sum);

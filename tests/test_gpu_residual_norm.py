@@ -360,3 +360,17 @@ def test_no_scale_touches_the_entry_to_the_first_block(kind, channels):
     _near(got[0][1], want, size, "dr")
     for other in got[1:]:
         assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("gate", [(3, 1, 96), (1, 96), (96,)])
+def test_the_gate_of_no_rows_has_a_gradient_of_zero(gate, dtype):
+    """Sequences without rows leave a gate of each sequence, or of all rows, as it is: nothing has used it."""
+    m = GatedResidualNorm(96, gate="linear")
+    empty = torch.empty(3, 0, 96, dtype=dtype, device="cuda")
+    table = [empty, empty.clone(), torch.ones(gate, dtype=dtype, device="cuda")]
+    for _ in range(2):
+        m.updateOutput(table)
+        dgate = m.backward(table, [empty, empty])[2]
+        assert dgate.shape == torch.Size(gate) and not dgate.any()
+        dgate.fill_(float("nan"))

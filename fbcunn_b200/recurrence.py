@@ -99,7 +99,8 @@ class GatedLinearRecurrence:
         if key != self._step_key:
             assert x.dim() == 2, "a step takes (sequences, channels)"
             self._check_table(x, g, z)
-            self._step_desc = self._new_desc(x, g, z, None, x.shape[0], 1)
+            desc = self._new_desc(x, g, z, None, x.shape[0], 1)
+            self._step_key, self._step_desc = None, desc  # no key until all that belongs to it is there
             self._step_ref = ctypes.byref(self._step_desc)
             if self._step_captured:
                 self._graphs.append(self._step_output)
@@ -171,14 +172,15 @@ class GatedLinearRecurrence:
                 assert offsets.dim() == 1 and offsets.numel() >= 1 and offsets.device == x.device and offsets.is_contiguous()
                 assert offsets.dtype in (torch.int32, torch.int64), "offsets are int32 or int64"
                 sequences, length = offsets.numel() - 1, 0
-            self._desc = self._new_desc(x, g, z, offsets, sequences, length)
+            desc = self._new_desc(x, g, z, offsets, sequences, length)
+            self._key, self._desc = None, desc  # no key until all that belongs to it is there
             self._desc_ref = ctypes.byref(self._desc)
             self._where, self._index = x.device, _device_index(x.device)
             self._made = _raw_stream(self._index)
             if self._captured:
                 self._graphs.append((self._output, self._state, self._checkpoints, self._grads, self._workspace, self._grad_state))
             self._captured = _capturing()
-            self._workspace = self._grad_state = None
+            self._workspace = self._grad_state = self._output = self._state = None
             self._output = torch.empty(x.shape, dtype=x.dtype, device=x.device)
             self._state = torch.empty((sequences, self.channels), dtype=torch.float32, device=x.device)
             self._checkpoints = self._grads = None
@@ -205,10 +207,10 @@ class GatedLinearRecurrence:
         parts = 3 if self.outputGate else 2
         if self._grads is None:
             self._projection = torch.empty(x.shape[:-1] + (parts * self.channels,), dtype=x.dtype, device=x.device)
-            self._grads = list(self._projection.split(self.channels, -1))
             n = int(capi.lib().fbfftconv_recurrence_workspace_bytes(self._desc_ref))
             self._workspace = torch.empty(max(n, 16), dtype=torch.uint8, device=x.device)
             self._grad_state = torch.empty_like(self._state)
+            self._grads = list(self._projection.split(self.channels, -1))
             self._made = self._made if _raw_stream(self._index) == self._made else -1  # of two streams: recorded on any
             self._desc.grad_x_stride = self._desc.grad_g_stride = self._desc.grad_z_stride = parts * self.channels
         self._desc.grad_y_stride = _row_stride(gradOutput)

@@ -147,16 +147,18 @@ class GatedResidualNorm:
             assert gate.dtype == kind, "the gate has the block's type"
             gate_rows = self._gate_rows(gate.shape[:-1], r.shape[:-1])
         types = capi.element_types()
-        self._desc = capi.NormDesc(
+        desc = capi.NormDesc(
             rows, gate_rows, _row_stride(u), _row_stride(r), _row_stride(gate), self.channels, types[kind],
             types[r.dtype], _NORMS[self.post], _NORMS[self.pre], _GATES[self.gate], self.eps, self.residualScale,
             self.branchScale, _device_index(r.device))
+        self._key, self._desc = None, desc  # no key until all that belongs to it is there
         self._desc_ref = ctypes.byref(self._desc)
         self._where, self._index, self._forward = r.device, _device_index(r.device), capi.lib().fbfftconv_residual_norm
         self._made = _raw_stream(self._index)
         if self._captured:
             self._graphs.append((self._r_out, self._v, self._stats, self._grads, self._workspace))
         self._captured = _capturing()
+        self._r_out = self._v = self._stats = None
         self._r_out = torch.empty(r.shape, dtype=r.dtype, device=r.device) if u is not None else None
         self._v = torch.empty(r.shape, dtype=kind, device=r.device) if self.pre is not None else None
         self._stats = torch.empty((rows, 4), dtype=torch.float32, device=r.device)
@@ -186,9 +188,9 @@ class GatedResidualNorm:
         assert kept is not None and self.stats is kept, "updateOutput of the same inputs runs first, in training() mode"
         grad_r, grad_v = self._grad_outputs(gradOutput, u, r)
         if self._grads is None:
-            self._grads = self._new_grads(u, r, gate)
             n = int(capi.lib().fbfftconv_residual_norm_workspace_bytes(self._desc_ref))
             self._workspace = torch.empty(max(n, 16), dtype=torch.uint8, device=r.device)
+            self._grads = self._new_grads(u, r, gate)
             self._made = self._made if _raw_stream(self._index) == self._made else -1  # of two streams: recorded on any
         du, dr, dgate = self._new_grads(u, r, gate) if scratch else self._grads
         weights = [_ptr(g) if parameters else None for g in (self.gradPostWeight, self.gradPostBias, self.gradPreWeight,

@@ -1,0 +1,145 @@
+"""What the modules of the sequence operators keep from call to call, on the host: their native calls are recorded, not
+made, and tensors of the host stand for the device's."""
+import ctypes
+
+import pytest
+import torch
+
+from fbcunn_b200 import AdamW, GatedLinearRecurrence, GatedResidualNorm, adamw, capi, module, recurrence, residual_norm
+
+
+class OnDevice(torch.Tensor):
+    """A tensor of the host that says it lies on the device."""
+    is_cuda = property(lambda self: True)
+
+
+class Host:
+    """Stands for the library and the stream: calls are (name, arguments), with descriptors and tables copied."""
+
+    def __init__(self):
+        self.calls, self.stream, self.capturing, self.recorded = [], 0, False, []
+
+    def __getattr__(self, name):
+        if not name.startswith("fbfftconv_"):
+            raise AttributeError(name)
+
+        def call(*args):
+            self.calls.append((name, [self._copy(a) for a in args]))
+            if name.endswith("_bytes"):
+                return 64
+            if name == "fbfftconv_adamw_create":
+                args[3]._obj.value = 1
+            return 0
+        return call
+
+    @staticmethod
+    def _copy(a):
+        value = getattr(a, "_obj", a)
+        if isinstance(value, ctypes.Structure):
+            return type(value).from_buffer_copy(value)
+        if isinstance(value, ctypes.Array):
+            return [type(t).from_buffer_copy(t) for t in value]
+        return value
+
+    def last(self, name):
+        return next(args for n, args in reversed(self.calls) if n == name)
+
+
+@pytest.fixture
+def host(monkeypatch):
+    h = Host()
+    monkeypatch.setattr(capi, "lib", lambda: h)
+    for m in (module, recurrence, residual_norm, adamw):
+        for name, value in (("_raw_stream", lambda index: h.stream), ("_stream", lambda device: h.stream),
+                            ("_capturing", lambda: h.capturing), ("_device_index", lambda device: 0)):
+            if hasattr(m, name):
+                monkeypatch.setattr(m, name, value)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda index=None: h.stream)
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, stream: h.recorded.append((t.data_ptr(), stream)))
+    return h
+
+
+def made(*shape, dtype=torch.float32):
+    return torch.ones(shape, dtype=dtype).as_subclass(OnDevice)
+
+
+def recurrent(channels=8, **kw):
+    return GatedLinearRecurrence(channels, device="cpu", **kw)
+
+
+def norm(channels=8, **kw):
+    return GatedResidualNorm(channels, device="cpu", **kw)
+
+
+def recurrence_table(n, length=3, channels=8):
+    return [made(n, length, channels) for _ in range(3)]
+
+
+def norm_table(n, channels=8):
+    return [made(n, channels) for _ in range(2)]
+
+
+CALLS = [  # (module, table of n rows or sequences, the call, the native entry, the descriptor's field that has n)
+    (recurrent, recurrence_table, lambda m, t: m.updateOutput(t), "fbfftconv_recurrence", "sequences"),
+    (recurrent, lambda n: [made(n, 8) for _ in range(3)], lambda m, t: m.step(t, made(t[0].shape[0], 8)),
+     "fbfftconv_recurrence_step", "sequences"),
+    (norm, norm_table, lambda m, t: m.updateOutput(t), "fbfftconv_residual_norm", "rows")]
+
+
+def _no_memory(monkeypatch, after):
+    """Allocations fail from the `after`-th on."""
+    left = [after]
+
+    def failing(make):
+        def call(*args, **kw):
+            left[0] -= 1
+            if left[0] < 0:
+                raise torch.OutOfMemoryError("no memory")
+            return make(*args, **kw)
+        return call
+    for name in ("empty", "empty_like"):
+        monkeypatch.setattr(torch, name, failing(getattr(torch, name)))
+
+
+@pytest.mark.parametrize("which", range(len(CALLS)))
+@pytest.mark.parametrize("after", [0, 1, 2])
+def test_a_call_that_found_no_memory_leaves_nothing_behind(host, monkeypatch, which, after):
+    """What a call of the first shape launches after a larger one has failed is described as it is, with tensors of its
+    size."""
+    build, table, call, entry, field = CALLS[which]
+    m, small, large = build(), table(2), table(500)
+    call(m, small)
+    with monkeypatch.context() as patch:
+        _no_memory(patch, after)
+        try:
+            call(m, large)
+        except torch.OutOfMemoryError:
+            pass
+    for t in (small, large, small):
+        out = call(m, t)
+        assert getattr(host.last(entry)[0], field) == t[0].shape[0]
+        out = out[0] if isinstance(out, list) else out
+        assert out.shape == t[0].shape
+        tensors = [v for v in vars(m).values() if isinstance(v, torch.Tensor)]
+        assert out.data_ptr() in host.last(entry) and any(v.data_ptr() == out.data_ptr() for v in tensors)
+
+
+@pytest.mark.parametrize("build,table,grads", [
+    (recurrent, recurrence_table, lambda t: t[0]), (norm, norm_table, lambda t: t)])
+def test_a_refused_call_or_one_without_memory_leaves_the_backward_pass(host, monkeypatch, build, table, grads):
+    m, t = build(), table(2)
+    m.updateOutput(t)
+    with pytest.raises(AssertionError):
+        m.updateOutput([x[..., :4] for x in t])
+    for after in (0, 1, 2):
+        with monkeypatch.context() as patch:
+            _no_memory(patch, after)
+            with pytest.raises(torch.OutOfMemoryError):
+                m.backward(t, grads(t))
+        assert not any(name.endswith("_backward") for name, _ in host.calls)
+    got = m.backward(t, grads(t))
+    assert all(g.shape == x.shape for g, x in zip(got, t))
+    name, args = host.calls[-1]
+    assert name.endswith("_backward") and all(g.data_ptr() in args for g in got)
+    if build is recurrent:
+        assert args[0].grad_x_stride == args[0].grad_z_stride == 24

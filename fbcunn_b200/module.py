@@ -66,6 +66,18 @@ def _layout(t: Optional[torch.Tensor]):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
 
+def _place(t: Optional[torch.Tensor]):
+    """Where a learned tensor lies: one that has been replaced, or whose storage has, lies elsewhere and is looked at anew."""
+    return None if t is None else (t.data_ptr(), t.nbytes)
+
+
+def _check_parameter(t: Optional[torch.Tensor], channels: int, device) -> None:
+    """A learned tensor of a sequence module, or its gradient."""
+    assert t is None or (isinstance(t, torch.Tensor) and t.device == device and t.dtype == torch.float32 and
+                         t.numel() == channels and t.is_contiguous()), \
+        "parameters and their gradients are fp32 (channels), contiguous and on the inputs' device"
+
+
 def _stream(device) -> int:
     """The current stream of a device as the integer the C ABI takes."""
     return _raw_stream(_device_index(device))

@@ -16,7 +16,7 @@ import math
 import torch
 
 from . import capi
-from .module import _capturing, _device_index, _layout, _ptr, _raw_stream, _stream, _used_here
+from .module import _capturing, _check_parameter, _device_index, _layout, _place, _ptr, _raw_stream, _stream, _used_here
 from .residual_norm import _row_stride
 
 
@@ -42,6 +42,7 @@ class GatedLinearRecurrence:
         self.output = self.state = self.gradInput = self.gradProjection = self.gradState = self.checkpoints = None
         self._key = None
         self._step_key = None
+        self._bias_place = self._grad_place = None  # of the bias and its gradient when they were looked at
         # whether a captured graph uses the tensors that are kept for the present shapes, and such tensors of earlier
         # shapes: a graph may be replayed after other shapes have run
         self._captured = self._step_captured = False
@@ -95,7 +96,10 @@ class GatedLinearRecurrence:
     def step(self, input, state):
         """One token: x, g and z are (sequences, channels), the states are updated in place."""
         x, g, z = self._table(input)
-        key = (_layout(x), _layout(g), _layout(z), id(self.bias))
+        key = (_layout(x), _layout(g), _layout(z))
+        bias = self.bias
+        if bias is not None and (bias.data_ptr(), bias.nbytes) != self._bias_place:  # _place, written out
+            self._check_bias(x)
         if key != self._step_key:
             assert x.dim() == 2, "a step takes (sequences, channels)"
             self._check_table(x, g, z)
@@ -110,11 +114,13 @@ class GatedLinearRecurrence:
             self._step_key, self._step_made = key, _raw_stream(self._step_index)
         if not self._step_captured:
             self._step_captured = _capturing()
-        _used_here(self._step_index, self._step_made, (self._step_output,))
+        stream = _raw_stream(self._step_index)
+        if stream != self._step_made:
+            _used_here(self._step_index, self._step_made, (self._step_output,))
         assert state.shape == x.shape and state.dtype == torch.float32 and state.is_contiguous() and state.is_cuda
         status = self._step_call(
-            self._step_ref, x.data_ptr(), g.data_ptr(), _ptr(z), _ptr(self.bias), state.data_ptr(),
-            self._step_output.data_ptr(), _raw_stream(self._step_index))
+            self._step_ref, x.data_ptr(), g.data_ptr(), _ptr(z), None if bias is None else self._bias_place[0], state.data_ptr(),
+            self._step_output.data_ptr(), stream)
         if status:
             capi.check(status)
         return self._step_output
@@ -142,9 +148,11 @@ class GatedLinearRecurrence:
             assert isinstance(t, torch.Tensor) and t.is_cuda and t.device == x.device, "CUDA support only!"
             assert t.dtype in capi.element_types() and t.dtype == x.dtype, "x, g and z have one type: fp32, bf16 or fp16"
             assert t.shape == x.shape and t.shape[-1] == self.channels, "size mismatch"
-        if self.bias is not None:
-            assert self.bias.device == x.device and self.bias.dtype == torch.float32 and self.bias.is_contiguous()
-            assert self.bias.numel() == self.channels
+        self._check_bias(x)
+
+    def _check_bias(self, x):
+        _check_parameter(self.bias, self.channels, x.device)
+        self._bias_place = _place(self.bias)
 
     def _new_desc(self, x, g, z, offsets, sequences, length):
         rows = math.prod(x.shape[:-1])
@@ -156,7 +164,9 @@ class GatedLinearRecurrence:
     def _prepare(self, input, offsets):
         """Checks the table; descriptor and outputs are kept for one set of shapes."""
         x, g, z = self._table(input)
-        key = (_layout(x), _layout(g), _layout(z), _layout(offsets), id(self.bias))
+        key = (_layout(x), _layout(g), _layout(z), _layout(offsets))
+        if _place(self.bias) != self._bias_place:
+            self._check_bias(x)
         if key == self._key:
             if not self._captured:
                 self._captured = _capturing()
@@ -221,6 +231,9 @@ class GatedLinearRecurrence:
             self._grad_state = torch.empty_like(self._grad_state)
         grads = [_ptr(t) if inputs else None for t in self._grads] + [None] * (3 - parts)
         with_bias = parameters and self.gradBias is not None
+        if with_bias and _place(self.gradBias) != self._grad_place:
+            _check_parameter(self.gradBias, self.channels, x.device)
+            self._grad_place = _place(self.gradBias)
         capi.check(capi.lib().fbfftconv_recurrence_backward(
             self._desc_ref, x.data_ptr(), g.data_ptr(), _ptr(z), _ptr(self.bias), _ptr(state), kept.data_ptr(),
             gradOutput.data_ptr(), _ptr(gradState), *grads, self._grad_state.data_ptr() if states else None,

@@ -17,7 +17,7 @@ import math
 import torch
 
 from . import capi
-from .module import _capturing, _device_index, _layout, _ptr, _raw_stream, _stream, _used_here
+from .module import _capturing, _check_parameter, _device_index, _layout, _place, _ptr, _raw_stream, _stream, _used_here
 
 _NORMS = {None: capi.NORM_NONE, "rms": capi.NORM_RMS, "layer": capi.NORM_LAYER}
 _GATES = {None: capi.GATE_NONE, "linear": capi.GATE_LINEAR, "sigmoid": capi.GATE_SIGMOID}
@@ -60,6 +60,7 @@ class GatedResidualNorm:
         self.stats = None
         self._key = None
         self._workspace = None
+        self._places = self._grad_places = self._weights = None  # of the weights and gradients when they were looked at
         self._captured = False  # whether a captured graph uses the tensors that are kept for the present shapes
         self._graphs = []       # such tensors of earlier shapes: a graph may be replayed after other shapes have run
 
@@ -85,8 +86,8 @@ class GatedResidualNorm:
         stats = self._stats if self.train else None
         self.stats = stats
         status = self._forward(
-            self._desc_ref, _ptr(u), r.data_ptr(), _ptr(gate), _ptr(self.postWeight), _ptr(self.postBias),
-            _ptr(self.preWeight), _ptr(self.preBias), _ptr(r_out), _ptr(v), _ptr(stats), _raw_stream(self._index))
+            self._desc_ref, _ptr(u), r.data_ptr(), _ptr(gate), *self._weights, _ptr(r_out), _ptr(v), _ptr(stats),
+            _raw_stream(self._index))
         if status:
             capi.check(status)
         self.output = v if u is None else r_out if v is None else [r_out, v]
@@ -121,12 +122,19 @@ class GatedResidualNorm:
     def _prepare(self, input):
         """Checks the table; descriptor and outputs are kept for one set of shapes."""
         u, r, gate = self._table(input)
-        key = (_layout(u), _layout(r), _layout(gate), self.residualScale, self.branchScale, self.eps, id(self.postWeight),
-               id(self.postBias), id(self.preWeight), id(self.preBias))
+        key = (_layout(u), _layout(r), _layout(gate), self.residualScale, self.branchScale, self.eps)
+        w1, b1, w2, b2 = self.postWeight, self.postBias, self.preWeight, self.preBias
+        # _place of each, written out: small calls are bound by what the host does
+        places = (w1 if w1 is None else (w1.data_ptr(), w1.nbytes), b1 if b1 is None else (b1.data_ptr(), b1.nbytes),
+                  w2 if w2 is None else (w2.data_ptr(), w2.nbytes), b2 if b2 is None else (b2.data_ptr(), b2.nbytes))
+        if places != self._places:
+            self._check_weights(r)
+            self._places, self._weights = places, tuple(_ptr(w) for w in (w1, b1, w2, b2))
         if key == self._key:
             if not self._captured:
                 self._captured = _capturing()
-            _used_here(self._index, self._made, (self._r_out, self._v, self._stats, self._workspace, *(self._grads or ())))
+            if _raw_stream(self._index) != self._made:
+                _used_here(self._index, self._made, (self._r_out, self._v, self._stats, self._workspace, *(self._grads or ())))
             return u, r, gate
         for t in (u, r, gate):
             if t is None:
@@ -135,8 +143,7 @@ class GatedResidualNorm:
             assert t.device == r.device, "tensors of two devices"
             assert t.dtype in capi.element_types(), "fp32, bf16 or fp16"
             assert t.dim() >= 1 and t.shape[-1] == self.channels, "channels mismatch"
-        for w in self.parameters()[0]:
-            assert w.device == r.device and w.dtype == torch.float32 and w.is_contiguous() and w.numel() == self.channels
+        self._check_weights(r)
         kind = r.dtype if u is None else u.dtype
         rows = math.prod(r.shape[:-1])
         gate_rows = 0
@@ -167,6 +174,10 @@ class GatedResidualNorm:
         self.stats = None
         return u, r, gate
 
+    def _check_weights(self, r):
+        for w in (self.postWeight, self.postBias, self.preWeight, self.preBias):
+            _check_parameter(w, self.channels, r.device)
+
     @staticmethod
     def _gate_rows(gate, rows):
         """Rows of a gate whose leading dimensions are those of the rows up to some place and 1 from there on."""
@@ -193,11 +204,18 @@ class GatedResidualNorm:
             self._grads = self._new_grads(u, r, gate)
             self._made = self._made if _raw_stream(self._index) == self._made else -1  # of two streams: recorded on any
         du, dr, dgate = self._new_grads(u, r, gate) if scratch else self._grads
-        weights = [_ptr(g) if parameters else None for g in (self.gradPostWeight, self.gradPostBias, self.gradPreWeight,
-                                                             self.gradPreBias)]
+        weights = [None] * 4
+        if parameters:
+            gradients = (self.gradPostWeight, self.gradPostBias, self.gradPreWeight, self.gradPreBias)
+            places = [_place(g) for g in gradients]
+            if places != self._grad_places:
+                for g in gradients:
+                    _check_parameter(g, self.channels, r.device)
+                self._grad_places = places
+            weights = [_ptr(g) for g in gradients]
         capi.check(capi.lib().fbfftconv_residual_norm_backward(
             self._desc_ref, _ptr(u), r.data_ptr(), _ptr(gate), kept.data_ptr(),
-            _ptr(self.postWeight), _ptr(self.postBias), _ptr(self.preWeight), _ptr(grad_r), _ptr(grad_v), _ptr(du),
+            *self._weights[:3], _ptr(grad_r), _ptr(grad_v), _ptr(du),
             dr.data_ptr(), _ptr(dgate), *weights, scale, int(self._accumulate), self._workspace.data_ptr(),
             self._workspace.numel(), _stream(self._where)))
         self.gradInput = dr if u is None else [du, dr] + ([dgate] if gate is not None else [])

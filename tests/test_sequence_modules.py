@@ -143,3 +143,61 @@ def test_a_refused_call_or_one_without_memory_leaves_the_backward_pass(host, mon
     assert name.endswith("_backward") and all(g.data_ptr() in args for g in got)
     if build is recurrent:
         assert args[0].grad_x_stride == args[0].grad_z_stride == 24
+
+
+STEPS = [lambda m, t: m.updateOutput(t), lambda m, t: m.step([x[:, 0] for x in t], made(2, 8))]
+REPLACED = {  # what may become of a parameter between two calls, and whether the call can still be made
+    "fewer": (lambda p: p[:3].clone(), False), "half": (lambda p: p.half(), False),
+    "apart": (lambda p: torch.zeros(16).as_subclass(OnDevice)[::2], False),
+    "other": (lambda p: torch.full_like(p, 2.0), True)}
+
+
+@pytest.mark.parametrize("as_data", [False, True])
+@pytest.mark.parametrize("how", REPLACED)
+def test_replaced_parameters_are_looked_at(host, how, as_data):
+    """As another tensor or in the same one; a sound one is used from then on, with the outputs that are there."""
+    make, sound = REPLACED[how]
+
+    def replace(m, name):
+        p = getattr(m, name)
+        new = make(p)
+        if as_data:
+            try:
+                p.data = new
+            except RuntimeError:  # of another type: not every version of the library allows that
+                pytest.skip("such a replacement is refused before it reaches the module")
+        else:
+            setattr(m, name, new)
+        return new
+
+    def used(call, address):
+        if not sound:
+            with pytest.raises(AssertionError):
+                call()
+            return
+        out = call()
+        assert address in host.calls[-1][1]
+        return out
+
+    for step in STEPS:
+        m, t = recurrent(), recurrence_table(2)
+        step(m, t)
+        new = replace(m, "bias")
+        used(lambda: step(m, t), new.data_ptr())
+    for name in ("postWeight", "preBias"):
+        m, t = norm(normBias=True), norm_table(2)
+        before = m.updateOutput(t)[0].data_ptr()
+        new = replace(m, name)
+        out = used(lambda: m.updateOutput(t), new.data_ptr())
+        assert not sound or out[0].data_ptr() == before
+    for name, m, t, dy in (("gradBias", recurrent(), recurrence_table(2), made(2, 3, 8)),
+                           ("gradPostWeight", norm(), norm_table(2), norm_table(2)),
+                           ("gradPreBias", norm(normBias=True), norm_table(2), norm_table(2))):
+        for again in (False, True):
+            m.updateOutput(t)
+            if again:
+                m.backward(t, dy)
+            new = replace(m, name)
+            used(lambda: m.backward(t, dy), new.data_ptr())
+            m.updateGradInput(t, dy)  # which does not touch it
+            setattr(m, name, made(8))

@@ -28,7 +28,8 @@ class GatedLinearRecurrence:
     apart); gradInput is laid out like that, as parts of one tensor, `gradProjection`.  states are fp32 (sequences,
     channels): the one after the last row of each sequence is left in `state`, the gradient by the initial one in
     gradState.  In training() mode, the default, updateOutput leaves in `checkpoints` what backward needs besides its
-    inputs, and backward must follow the updateOutput of the same inputs.  gradBias is overwritten, or added to with
+    inputs, and backward must follow the updateOutput of the same inputs.  An output or state that is given back as an
+    input is the caller's from then on: the call makes others.  gradBias is overwritten, or added to with
     accumulate=True."""
 
     def __init__(self, channels, *, outputGate=True, bias=True, device="cuda", accumulate=False):
@@ -73,10 +74,12 @@ class GatedLinearRecurrence:
         rows, of which those outside of all sequences stay as they are in `output`."""
         x, g, z = self._prepare(input, offsets)
         self._check_state(state, "initial state")
+        # what was returned before is an input now
         if state is not None and state.data_ptr() == self._state.data_ptr():
-            if self._captured:
-                self._graphs.append(self._state)
-            self._state = torch.empty_like(self._state)  # what was returned before is an input now
+            self._state = self._another(self._state)
+        output = self._output.data_ptr()
+        if x.data_ptr() == output or g.data_ptr() == output or _ptr(z) == output:
+            self._output = self._another(self._output)
         checkpoints = None
         if self.train:
             if self._checkpoints is None:
@@ -206,6 +209,12 @@ class GatedLinearRecurrence:
                 f"the {what} is fp32 (sequences, channels)"
             assert state.device == self._where, "CUDA support only!"
 
+    def _another(self, t):
+        """A tensor in the place of one that the module has given away."""
+        if self._captured:
+            self._graphs.append(t)
+        return torch.empty_like(t)
+
     def _backward(self, input, gradOutput, scale, state, offsets, gradState, inputs, parameters):
         kept = self.checkpoints
         x, g, z = self._prepare(input, offsets)
@@ -226,9 +235,7 @@ class GatedLinearRecurrence:
         self._desc.grad_y_stride = _row_stride(gradOutput)
         states = inputs and (state is not None or gradState is not None)
         if states and gradState is not None and gradState.data_ptr() == self._grad_state.data_ptr():
-            if self._captured:
-                self._graphs.append(self._grad_state)
-            self._grad_state = torch.empty_like(self._grad_state)
+            self._grad_state = self._another(self._grad_state)
         grads = [_ptr(t) if inputs else None for t in self._grads] + [None] * (3 - parts)
         with_bias = parameters and self.gradBias is not None
         if with_bias and _place(self.gradBias) != self._grad_place:

@@ -32,7 +32,7 @@ class GatedResidualNorm:
     for one of all rows.  Without post-norm and gate the table may be [r] (or r itself): v = pre(r), the entry to the
     first block, which no scale touches.  Without pre-norm the output is r'.  Weights are fp32; in training() mode, the default, updateOutput
     leaves in `stats` what backward needs besides its inputs, and backward must follow the updateOutput of the same
-    inputs.  Gradients of weights are overwritten, or added to with accumulate=True."""
+    inputs.  An output that is given back as an input is the caller's from then on: the call makes another.  Gradients of weights are overwritten, or added to with accumulate=True."""
 
     def __init__(self, channels, *, post="rms", pre="rms", gate=None, residualScale=1.0, branchScale=1.0, normBias=False,
                  eps=1e-6, device="cuda", accumulate=False):
@@ -82,15 +82,17 @@ class GatedResidualNorm:
 
     def updateOutput(self, input):
         u, r, gate = self._prepare(input)
-        r_out, v = self._r_out, self._v
         stats = self._stats if self.train else None
         self.stats = stats
+        inputs = _ptr(u), r.data_ptr(), _ptr(gate)
+        if self._r_at in inputs or self._v_at in inputs:
+            self._give_away(inputs)
         status = self._forward(
-            self._desc_ref, _ptr(u), r.data_ptr(), _ptr(gate), *self._weights, _ptr(r_out), _ptr(v), _ptr(stats),
-            _raw_stream(self._index))
+            self._desc_ref, *inputs, *self._weights, self._r_at if self._r_at > 0 else None,
+            self._v_at if self._v_at > 0 else None, _ptr(stats), _raw_stream(self._index))
         if status:
             capi.check(status)
-        self.output = v if u is None else r_out if v is None else [r_out, v]
+        self.output = self._v if u is None else self._r_out if self._v is None else [self._r_out, self._v]
         return self.output
 
     def forward(self, input):
@@ -170,9 +172,24 @@ class GatedResidualNorm:
         self._v = torch.empty(r.shape, dtype=kind, device=r.device) if self.pre is not None else None
         self._stats = torch.empty((rows, 4), dtype=torch.float32, device=r.device)
         self._grads = self._workspace = None
+        self._set_outputs()
         self._key = key
         self.stats = None
         return u, r, gate
+
+    def _give_away(self, inputs):
+        """Other outputs in the place of those that were returned before and are inputs now."""
+        if self._captured:
+            self._graphs.append((self._r_out, self._v))
+        if self._r_at in inputs:
+            self._r_out = torch.empty_like(self._r_out)
+        if self._v_at in inputs:
+            self._v = torch.empty_like(self._v)
+        self._set_outputs()
+
+    def _set_outputs(self):
+        """Where the outputs lie; -1 for those that are not there or have no elements."""
+        self._r_at, self._v_at = _ptr(self._r_out) or -1, _ptr(self._v) or -1
 
     def _check_weights(self, r):
         for w in (self.postWeight, self.postBias, self.preWeight, self.preBias):

@@ -536,3 +536,12 @@ def test_output_gates_that_are_masked(dtype):
     dx, dg, dz = m.backward(table, one * 2.0 ** -20)
     assert all(torch.isfinite(g).all() for g in (dx, dg, dz))
     assert ((dz[0, :, 0].double() - h * 2.0 ** -20).abs() <= torch.finfo(dtype).eps * h * 2.0 ** -20 + 2.0 ** -25).all()
+
+
+def test_one_module_in_several_layers():
+    """A module that is shared by layers takes its own output in."""
+    m, table, dy, h0, dlast = make((2, 50), 2, 32, F32, seed=14)
+    y = m.updateOutput(table, state=h0)
+    want = y.clone()
+    check(m, [y, *table[1:]], dy, h0, dlast)
+    assert torch.equal(y, want)

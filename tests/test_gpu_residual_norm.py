@@ -374,3 +374,17 @@ def test_the_gate_of_no_rows_has_a_gradient_of_zero(gate, dtype):
         dgate = m.backward(table, [empty, empty])[2]
         assert dgate.shape == torch.Size(gate) and not dgate.any()
         dgate.fill_(float("nan"))
+
+
+def test_one_module_at_several_borders():
+    """A module that is shared by blocks takes its own outputs in; each backward pass has the inputs that it was given."""
+    m, (u, r), grads = build((6,), 96, F32)
+    twin, *_ = build((6,), 96, F32)
+    r1, v1 = m.updateOutput([u, r])
+    want = [t.clone() for t in (r1, v1)]
+    second = m.updateOutput([v1, r1])
+    assert torch.equal(r1, want[0]) and torch.equal(v1, want[1])
+    got = [t.clone() for t in second + m.backward([v1, r1], grads)]
+    table = want[::-1]
+    for a, b in zip(got, twin.updateOutput(table) + twin.backward(table, grads)):
+        assert torch.equal(a, b)

@@ -201,3 +201,38 @@ def test_replaced_parameters_are_looked_at(host, how, as_data):
             used(lambda: m.backward(t, dy), new.data_ptr())
             m.updateGradInput(t, dy)  # which does not touch it
             setattr(m, name, made(8))
+
+
+def test_outputs_that_are_given_back_stay_what_they_are(host):
+    """A module that is applied again to what it returned writes to other tensors."""
+    m, t = recurrent(), recurrence_table(2)
+    for place in range(3):
+        t[place] = m.updateOutput(t).as_subclass(OnDevice)
+        again = m.updateOutput(t)
+        assert again.data_ptr() != t[place].data_ptr() and again.data_ptr() in host.calls[-1][1]
+        assert m.output is again and again.shape == t[place].shape
+    m, t = norm(gate="linear"), norm_table(2) + [made(2, 8)]
+    for place in range(3):
+        for which in range(2):
+            t[place] = m.updateOutput(t)[which].as_subclass(OnDevice)
+            again = m.updateOutput(t)
+            assert all(a.data_ptr() in host.calls[-1][1] for a in again)
+            assert not {a.data_ptr() for a in again} & {x.data_ptr() for x in t}
+    kept = [a.data_ptr() for a in m.updateOutput([x.clone() for x in t])]
+    assert kept == [a.data_ptr() for a in m.updateOutput([x.clone() for x in t])]  # else the same ones are used again
+    entry = norm(post=None)
+    v = entry.updateOutput(made(2, 8)).as_subclass(OnDevice)
+    assert entry.updateOutput(v).data_ptr() != v.data_ptr()
+    for m, t in ((entry, [made(0, 8)]), (norm(), norm_table(0)), (norm(pre=None), norm_table(0)), (recurrent(), recurrence_table(0))):
+        out = m.updateOutput(t)
+        assert (out[-1] if isinstance(out, list) else out).numel() == 0 and m.updateOutput(t) is not None
+
+
+def test_outputs_of_a_captured_graph_that_are_given_back_are_kept(host):
+    host.capturing = True
+    for m, t, at in ((recurrent(), recurrence_table(2), 0), (norm(), norm_table(2), 1)):
+        out = m.updateOutput(t)
+        out = out[0] if isinstance(out, list) else out
+        t[at] = out.as_subclass(OnDevice)
+        m.updateOutput(t)
+        assert any(k is out for kept in m._graphs for k in (kept if isinstance(kept, tuple) else (kept,)))

@@ -213,6 +213,7 @@ class GatedLinearRecurrence:
         """A tensor in the place of one that the module has given away."""
         if self._captured:
             self._graphs.append(t)
+        self._made = self._made if _raw_stream(self._index) == self._made else -1  # of two streams: recorded on any
         return torch.empty_like(t)
 
     def _backward(self, input, gradOutput, scale, state, offsets, gradState, inputs, parameters):

@@ -185,6 +185,7 @@ class GatedResidualNorm:
             self._r_out = torch.empty_like(self._r_out)
         if self._v_at in inputs:
             self._v = torch.empty_like(self._v)
+        self._made = self._made if _raw_stream(self._index) == self._made else -1  # of two streams: recorded on any
         self._set_outputs()
 
     def _set_outputs(self):

@@ -236,3 +236,33 @@ def test_outputs_of_a_captured_graph_that_are_given_back_are_kept(host):
         t[at] = out.as_subclass(OnDevice)
         m.updateOutput(t)
         assert any(k is out for kept in m._graphs for k in (kept if isinstance(kept, tuple) else (kept,)))
+
+
+def test_what_was_made_on_another_stream_in_between_is_recorded(host):
+    """Tensors that were made anew on stream 2, in the place of some of stream 1, are recorded when stream 1 uses them."""
+    def swap_state(m, t):
+        m.updateOutput(t, state=m.state)
+
+    def swap_output(m, t):
+        m.updateOutput([m.output] + t[1:])
+
+    def swap_grad_state(m, t):
+        m.updateOutput(t)
+        m.backward(t, t[0], gradState=m.gradState)
+
+    cases = [(recurrent, recurrence_table, swap_state, lambda m: m.state),
+             (recurrent, recurrence_table, swap_output, lambda m: m.output),
+             (recurrent, recurrence_table, swap_grad_state, lambda m: m.gradState),
+             (norm, norm_table, lambda m, t: m.updateOutput([t[0], m.output[0]]), lambda m: m.output[0])]
+    for build, table, swap, what in cases:
+        host.stream = 1
+        m, t = build(), table(2)
+        m.updateOutput(t)
+        if build is recurrent:
+            m.backward(t, t[0], state=made(2, 8), gradState=made(2, 8))
+        host.stream = 2
+        swap(m, t)
+        new = what(m).data_ptr()
+        host.stream, host.recorded = 1, []
+        m.updateOutput(t)
+        assert (new, 1) in host.recorded

@@ -7,6 +7,7 @@ can be captured into a CUDA graph and replayed.
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import torch
 
@@ -14,6 +15,9 @@ from . import capi
 from .module import _device_index, _stream
 
 _BLOCK = 256  # elements that share a scale
+
+# of every tensor at every step: what has another address or size is looked at anew
+_address, _nbytes = torch.Tensor.data_ptr, operator.attrgetter("nbytes")
 
 
 class AdamW:
@@ -26,7 +30,8 @@ class AdamW:
     seed           of the random rounding of 8-bit moments
 
     Tensors are contiguous and on one GPU; gradients have their parameter's shape and any of the three types.
-    A tensor whose storage has been replaced since the last step is noticed and used from then on."""
+    A tensor whose storage has been replaced since the last step is noticed and used from then on, if it is still such
+    a tensor of as many elements."""
 
     def __init__(self, params, grads=None, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weightDecay=1e-2, *, stateBits=32,
                  min8bitSize=4096, masters=None, seed=0):
@@ -51,10 +56,8 @@ class AdamW:
             masters = [None if p.dtype == torch.float32 else p.detach().float().contiguous() for p in self.params]
         self.masters = list(masters) if masters is not None else [None] * len(self.params)
         assert len(self.masters) == len(self.params), "one master for each parameter"
-        for p, g, w in zip(self.params, self.grads, self.masters):
-            assert g.shape == p.shape, "gradient size mismatch"
-            assert w is None or (w.is_cuda and w.shape == p.shape and w.dtype == torch.float32 and w.is_contiguous())
-            assert all(t.is_contiguous() and t.device == self.device and t.dtype in capi.element_types() for t in (p, g))
+        self._counts = [p.numel() for p in self.params]
+        self._check()
         # where each tensor's moments lie: (bits, first element) in the flat tensors, a tensor starts on a block
         size, self.layout = {8: 0, 32: 0}, []
         for p in self.params:
@@ -99,7 +102,8 @@ class AdamW:
             assert scalars.device == self.device and scalars.dtype == torch.float32 and scalars.numel() == 2
             assert scalars.is_contiguous()
             scalars = scalars.data_ptr()
-        if [t.data_ptr() for t in self._watched] != self._addresses:
+        if list(map(_address, self._watched)) != self._addresses or list(map(_nbytes, self._watched)) != self._sizes:
+            self._check()
             self._rebuild()
         capi.check(capi.lib().fbfftconv_adamw_step(
             self._handle, self.lr if lr is None else lr, gradScale, scalars, _stream(self.device)))
@@ -116,6 +120,13 @@ class AdamW:
         self._counter[0] = int(state["steps"])
 
     # -- internals -----------------------------------------------------------------
+    def _check(self):
+        for p, g, w, n in zip(self.params, self.grads, self.masters, self._counts):
+            assert p.numel() == n, "a parameter has another size than its moments"
+            assert g.shape == p.shape, "gradient size mismatch"
+            assert w is None or (w.device == self.device and w.shape == p.shape and w.dtype == torch.float32 and w.is_contiguous())
+            assert all(t.is_contiguous() and t.device == self.device and t.dtype in capi.element_types() for t in (p, g))
+
     def _rebuild(self):
         """The native handle for the tensors as they are now."""
         tensors = (capi.AdamwTensor * len(self.params))()
@@ -140,7 +151,7 @@ class AdamW:
         self._destroy()
         self._handle = handle
         self._watched = self.params + self.grads + [w for w in self.masters if w is not None]
-        self._addresses = [t.data_ptr() for t in self._watched]
+        self._addresses, self._sizes = list(map(_address, self._watched)), list(map(_nbytes, self._watched))
 
     def _destroy(self):
         if self._handle is not None:

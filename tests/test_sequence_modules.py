@@ -266,3 +266,60 @@ def test_what_was_made_on_another_stream_in_between_is_recorded(host):
         host.stream, host.recorded = 1, []
         m.updateOutput(t)
         assert (new, 1) in host.recorded
+
+
+def optimizer(sizes=(4, 600, 30), **kw):
+    params = [made(n) for n in sizes]
+    grads = [made(n) for n in sizes]
+    return AdamW(params, grads, **kw), params, grads
+
+
+def test_replaced_storage_of_optimized_tensors_is_looked_at(host):
+    """As long as a tensor fits its moments it may lie elsewhere; what does not is refused before anything is launched."""
+    opt, params, grads = optimizer(masters=[None] * 3)
+    params[1].data = made(600)
+    opt.step()
+    assert host.last("fbfftconv_adamw_create")[0][1].param == params[1].data_ptr()
+    fits, steps = {"param": params, "grad": grads}, sum(n == "fbfftconv_adamw_step" for n, _ in host.calls)
+    for which, tensors in fits.items():
+        for bad in (made(700), made(500), torch.zeros(1200).as_subclass(OnDevice)[::2], made(600).half().int(), made(20, 30)):
+            kept = tensors[1].data
+            try:
+                tensors[1].data = bad
+            except RuntimeError:
+                continue
+            if bad.shape == (20, 30) and which == "param":
+                grads[1].data = bad  # a shape of as many elements is no other size
+                opt.step()
+                steps += 1
+                grads[1].data = made(600)
+            else:
+                with pytest.raises(AssertionError):
+                    opt.step()
+                with pytest.raises(AssertionError):
+                    opt.step()  # it stays refused
+            tensors[1].data = kept
+            opt.step()
+            steps += 1
+            assert sum(n == "fbfftconv_adamw_step" for n, _ in host.calls) == steps
+
+
+def test_a_tensor_of_another_size_at_the_same_address_is_looked_at(host):
+    opt, params, grads = optimizer()
+    opt.step()
+    for tensors in (params, grads):
+        kept = tensors[2].data
+        tensors[2].data = kept[:10]
+        assert tensors[2].data_ptr() == kept.data_ptr()
+        with pytest.raises(AssertionError):
+            opt.step()
+        tensors[2].data = kept
+
+
+def test_masters_are_looked_at(host):
+    params, grads = [made(64, dtype=torch.bfloat16)], [made(64)]
+    opt = AdamW(params, grads, masters=[made(64)])
+    opt.step()
+    opt.masters[0].data = made(32)
+    with pytest.raises(AssertionError):
+        opt.step()

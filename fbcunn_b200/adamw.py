@@ -26,7 +26,8 @@ class AdamW:
     stateBits      32, or 8: e4m3 moments with a scale for every 256 elements, for tensors of at least
                    `min8bitSize` elements (smaller ones keep 32 bits: their codes would save nothing)
     masters        for 16-bit parameters: a list of fp32 tensors that are the weights themselves (adopted, not
-                   copied; None for fp32 parameters), or True to make them from the parameters
+                   copied; None for fp32 parameters), or True to make them from the parameters; those are part of
+                   state(), adopted ones are the caller's to save
     seed           of the random rounding of 8-bit moments
 
     Tensors are contiguous and on one GPU; gradients have their parameter's shape and any of the three types.
@@ -52,6 +53,7 @@ class AdamW:
         for t in self.params + self.grads:
             assert isinstance(t, torch.Tensor) and t.is_cuda, "CUDA support only!"
         self.device = self.params[0].device
+        self._own_masters = masters is True
         if masters is True:
             masters = [None if p.dtype == torch.float32 else p.detach().float().contiguous() for p in self.params]
         self.masters = list(masters) if masters is not None else [None] * len(self.params)
@@ -109,14 +111,30 @@ class AdamW:
             self._handle, self.lr if lr is None else lr, gradScale, scalars, _stream(self.device)))
 
     def state(self) -> dict:
-        """The moments and the step count, as loadState takes them."""
-        return dict({k: v.clone() for k, v in self.moments.items()}, steps=self.steps)
+        """The moments, the step count and the masters that were made here, as loadState takes them."""
+        state = dict({k: v.clone() for k, v in self.moments.items()}, steps=self.steps)
+        if self._own_masters:
+            state["masters"] = [None if w is None else w.clone() for w in self.masters]
+        return state
 
     def loadState(self, state):
-        assert set(state) == set(self.moments) | {"steps"}, "the state of other parameters"
-        for k, v in self.moments.items():
-            assert state[k].shape == v.shape and state[k].dtype == v.dtype, "the state of other parameters"
-            v.copy_(state[k])
+        """Takes up where state() was asked for.  Parameters with masters of the state become their rounded copies."""
+        masters = state.get("masters", []) if self._own_masters else []
+        assert set(state) == set(self.moments) | {"steps"} | ({"masters"} if self._own_masters else set()), \
+            "the state of other parameters, or of masters that are kept elsewhere"
+        assert not self._own_masters or len(masters) == len(self.masters), "the state of other parameters"
+        kept = [(self.moments[k], state[k]) for k in self.moments]
+        for w, saved in zip(self.masters, masters):
+            assert (w is None) == (saved is None), "the state of other parameters"
+            if w is not None:
+                kept.append((w, saved))
+        for t, saved in kept:
+            assert saved.shape == t.shape and saved.dtype == t.dtype, "the state of other parameters"
+        for t, saved in kept:
+            t.copy_(saved)
+        for p, w in zip(self.params, self.masters):
+            if self._own_masters and w is not None:
+                p.detach().copy_(w)
         self._counter[0] = int(state["steps"])
 
     # -- internals -----------------------------------------------------------------

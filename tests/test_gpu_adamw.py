@@ -355,3 +355,19 @@ def test_a_captured_step_of_many_tensors():
             b.step()
         assert a.steps == b.steps == 3
         assert all(torch.equal(p, q) for p, q in zip(a.params + a.masters, b.params + b.masters))
+
+
+def test_a_run_goes_on_from_its_state():
+    """Weights that live in masters made here are the state's: the steps after a resume are those of the run itself."""
+    params, grads, _ = _tensors([5000, 77], torch.bfloat16, torch.bfloat16)
+    a = AdamW(params, grads, stateBits=8, masters=True, seed=3, **HYPER)
+    for _ in range(3):
+        a.step()
+    saved = [p.clone() for p in params]
+    state = a.state()
+    a.step()
+    b = AdamW(saved, grads, stateBits=8, masters=True, seed=3, **HYPER)
+    b.loadState(state)
+    b.step()
+    for p, q in zip(a.params + a.masters, b.params + b.masters):
+        assert torch.equal(p, q)

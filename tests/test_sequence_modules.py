@@ -323,3 +323,29 @@ def test_masters_are_looked_at(host):
     opt.masters[0].data = made(32)
     with pytest.raises(AssertionError):
         opt.step()
+
+
+def test_the_state_has_the_masters_that_were_made_here(host):
+    def build(**kw):
+        params = [torch.full((40,), 1.0 + 2.0 ** -6, dtype=torch.bfloat16).as_subclass(OnDevice), made(8)]
+        return AdamW(params, [made(40), made(8)], **kw), params
+
+    opt, params = build(masters=True)
+    opt.masters[0].add_(2.0 ** -12)  # what 16 bits do not hold
+    state = opt.state()
+    assert state["masters"][1] is None and state["masters"][0].data_ptr() != opt.masters[0].data_ptr()
+    other, theirs = build(masters=True)
+    theirs[0].zero_()
+    other.loadState(state)
+    assert torch.equal(other.masters[0], opt.masters[0]) and torch.equal(theirs[0], opt.masters[0].bfloat16())
+    for bad in ({k: v for k, v in state.items() if k != "masters"}, dict(state, masters=state["masters"][:1]),
+                dict(state, masters=[None, None]), dict(state, masters=[state["masters"][0][:7], None])):
+        before = {k: v.clone() for k, v in other.moments.items()}
+        with pytest.raises(AssertionError):
+            other.loadState(bad)
+        assert all(torch.equal(before[k], v) for k, v in other.moments.items())
+    adopted, _ = build(masters=[made(40), None])
+    assert "masters" not in adopted.state()
+    adopted.loadState(adopted.state())
+    with pytest.raises(AssertionError):
+        adopted.loadState(state)

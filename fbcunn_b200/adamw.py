@@ -94,8 +94,12 @@ class AdamW:
         for p, g, old in zip(self.params, grads, self.grads):
             assert isinstance(g, torch.Tensor) and g.device == self.device and g.is_contiguous()
             assert g.shape == p.shape and g.dtype == old.dtype, "gradient size or type mismatch"
-        self.grads = grads
-        self._rebuild()
+        before, self.grads = self.grads, grads
+        try:
+            self._rebuild()
+        except capi.FbfftconvError:
+            self.grads = before
+            raise
 
     def step(self, lr=None, gradScale=1.0, scalars=None):
         """One step on the current stream.  gradScale multiplies the gradients; scalars, a tensor of two floats on the

@@ -474,8 +474,9 @@ int check_pointers(const fbfftconv_adamw_tensor& t, int device) {
   return FBFFTCONV_OK;
 }
 
-// What a step writes must not be written twice: a parameter that is listed twice would be updated by two warps at once.
-int check_overlap(const fbfftconv_adamw_tensor* tensors, int count) {
+// What a step writes must not be written twice, nor read as a gradient: a parameter that is listed twice would be updated
+// by two warps at once, and a gradient that lies in one be read before or after its update.
+int check_overlap(const fbfftconv_adamw_tensor* tensors, int count, const fbfftconv_adamw_options& options) {
   std::vector<std::pair<uintptr_t, uintptr_t>> written;
   const auto add = [&](const void* p, long long bytes) {
     if (p && bytes) written.emplace_back((uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes);
@@ -490,10 +491,19 @@ int check_overlap(const fbfftconv_adamw_tensor* tensors, int count) {
     add(t.scale1, 4ll * blocks_of(t.count));
     add(t.scale2, 4ll * blocks_of(t.count));
   }
+  add(options.steps, 2 * sizeof(int64_t));
   std::sort(written.begin(), written.end());
   for (size_t i = 1; i < written.size(); ++i)
     if (written[i].first < written[i - 1].second)
-      return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "parameters, masters and moments must not share memory");
+      return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "parameters, masters, moments and steps must not share memory");
+  for (int i = 0; i < count; ++i) {
+    const uintptr_t begin = (uintptr_t)tensors[i].grad;
+    const uintptr_t end = begin + (uintptr_t)(tensors[i].count * type_bytes(tensors[i].grad_type));
+    if (begin == end) continue;
+    const auto next = std::lower_bound(written.begin(), written.end(), std::make_pair(end, (uintptr_t)0));
+    if (next != written.begin() && (next - 1)->second > begin)  // the last one that begins before the gradient's end
+      return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "gradient %d must not share memory with what a step writes", i);
+  }
   return FBFFTCONV_OK;
 }
 
@@ -511,7 +521,7 @@ int create(const fbfftconv_adamw_tensor* tensors, int count, const fbfftconv_ada
   if (!o.steps || !aligned_to(o.steps, 8))
     return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "steps must name two 8-byte integers");
   for (int i = 0; i < count; ++i) OP_TRY(check_tensor(tensors[i], i));
-  OP_TRY(check_overlap(tensors, count));
+  OP_TRY(check_overlap(tensors, count, o));
   std::unique_ptr<fbfftconv_adamw> h(new fbfftconv_adamw);
   h->tensors.assign(tensors, tensors + count);
   h->options = o;
@@ -519,6 +529,22 @@ int create(const fbfftconv_adamw_tensor* tensors, int count, const fbfftconv_ada
   OP_TRY(validate_device_pointer(h->device, o.steps, "steps"));
   for (const auto& t : h->tensors) OP_TRY(check_pointers(t, h->device));
   *out = h.release();
+  return FBFFTCONV_OK;
+}
+
+int set_gradients(fbfftconv_adamw* h, const void* const* grads, int count) {
+  if (!h || count != (int)h->tensors.size() || (count && !grads))
+    return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "one gradient for each tensor");
+  std::vector<fbfftconv_adamw_tensor> tensors = h->tensors;
+  for (int i = 0; i < count; ++i) {
+    if (tensors[i].count == 0) continue;
+    if (!grads[i] || !aligned_to(grads[i], type_bytes(tensors[i].grad_type)))
+      return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "gradient %d is null or not aligned to its element", i);
+    OP_TRY(validate_device_pointer(h->device, grads[i], "a gradient"));
+    tensors[i].grad = grads[i];
+  }
+  OP_TRY(check_overlap(tensors.data(), count, h->options));
+  h->tensors.swap(tensors);
   return FBFFTCONV_OK;
 }
 
@@ -576,16 +602,11 @@ int fbfftconv_adamw_destroy(fbfftconv_adamw* h) {
 }
 
 int fbfftconv_adamw_set_gradients(fbfftconv_adamw* h, const void* const* grads, int count) {
-  if (!h || count != (int)h->tensors.size() || (count && !grads))
-    return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "one gradient for each tensor");
-  for (int i = 0; i < count; ++i) {
-    if (h->tensors[i].count == 0) continue;
-    if (!grads[i] || !aligned_to(grads[i], type_bytes(h->tensors[i].grad_type)))
-      return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "gradient %d is null or not aligned to its element", i);
-    OP_TRY(validate_device_pointer(h->device, grads[i], "a gradient"));
+  try {
+    return set_gradients(h, grads, count);
+  } catch (const std::bad_alloc&) {
+    return op_fail(FBFFTCONV_ERR_NOMEM, "out of host memory");
   }
-  for (int i = 0; i < count; ++i) h->tensors[i].grad = grads[i];
-  return FBFFTCONV_OK;
 }
 
 int fbfftconv_adamw_step(fbfftconv_adamw* h, double lr, float grad_scale, const float* scalars, fbfftconv_stream stream) {

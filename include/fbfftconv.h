@@ -328,7 +328,7 @@ enum { FBFFTCONV_FLOAT32 = 0, FBFFTCONV_BFLOAT16 = 1, FBFFTCONV_FLOAT16 = 2 };
  *
  * `master`, for 16-bit parameters, is the weight itself in fp32; param is then its rounded copy and is only written.
  * Every array is contiguous and aligned to its element; 16-byte alignment (8 for codes) is what the vector loads want.
- * Nothing that a step writes may overlap.  Tensors without elements are skipped. */
+ * Nothing that a step writes may overlap, nor a gradient lie in it.  Tensors without elements are skipped. */
 typedef struct fbfftconv_adamw fbfftconv_adamw;
 typedef struct fbfftconv_adamw_tensor {
   void* param;

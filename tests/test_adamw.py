@@ -62,3 +62,26 @@ def test_tensors_that_touch_do_not_overlap(lib):
     tensors = [_tensor(), _tensor(param=4096 + 64, grad=8192 + 64, moment1=12288 + 64, moment2=16384 + 64)]
     rc = _create(lib, tensors, _options())
     assert "share memory" not in capi.last_error() and rc in (capi.ERR_CUDA, capi.ERR_INVALID_ARGUMENT)
+
+
+@pytest.mark.parametrize("grad,message", [
+    (4096, "gradient"), (4096 + 60, "gradient"), (4096 - 60, "gradient"), (12288 + 32, "gradient"), (16384 + 60, "gradient"),
+    ((1 << 20) - 60, "gradient"), ((1 << 20) + 12, "gradient"), (4096 + 64, None), (4096 - 64, None), ((1 << 20) + 16, None)])
+def test_gradients_apart_from_what_is_written(lib, grad, message):
+    """A gradient that lies in a parameter, a moment or the count is refused, one beside them is not."""
+    rc = _create(lib, [_tensor(grad=grad)], _options())
+    if message:
+        assert rc == capi.ERR_INVALID_ARGUMENT and "share memory" in capi.last_error() and message in capi.last_error()
+    else:
+        assert "share memory" not in capi.last_error()
+
+
+def test_counts_apart_from_what_is_written(lib):
+    assert _create(lib, [_tensor()], _options(steps=4096 + 56)) == capi.ERR_INVALID_ARGUMENT
+    assert "share memory" in capi.last_error()
+
+
+def test_tensors_may_share_a_gradient(lib):
+    tensors = [_tensor(), _tensor(param=4096 + 64, moment1=12288 + 64, moment2=16384 + 64)]
+    _create(lib, tensors, _options())
+    assert "share memory" not in capi.last_error()

@@ -371,3 +371,20 @@ def test_a_run_goes_on_from_its_state():
     b.step()
     for p, q in zip(a.params + a.masters, b.params + b.masters):
         assert torch.equal(p, q)
+
+
+def test_gradients_that_lie_in_what_is_stepped_are_refused():
+    p, g = torch.zeros(300, device="cuda"), torch.zeros(300, device="cuda")
+    for grad in (p, p[:]):
+        with pytest.raises(capi.FbfftconvError, match="share memory"):
+            AdamW([p], [grad])
+    with pytest.raises(capi.FbfftconvError, match="share memory"):
+        AdamW([p[:200]], [p[100:]])
+    opt = AdamW([p], [g])
+    inside = (capi.c_void_p * 1)(opt.moments["m"].data_ptr())
+    assert capi.lib().fbfftconv_adamw_set_gradients(opt._handle, inside, 1) == capi.ERR_INVALID_ARGUMENT
+    with pytest.raises(capi.FbfftconvError, match="share memory"):
+        opt.setGradients([opt.moments["v"][:300]])
+    assert opt.grads[0] is g
+    opt.step()
+    assert opt.steps == 1

@@ -217,18 +217,23 @@ __device__ __forceinline__ float magnitude(const float (&x)[8]) {
   return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));  // NaN's bits are above infinity's
 }
 
-__device__ __forceinline__ float sqrt_fast(float v) {  // what is below the smallest normal number counts as zero
+// Flushed, what is below the smallest normal number counts as zero: a root that is then below 2^-63 is nothing beside eps,
+// unless eps is nearly as small (`small_eps`): then a kernel of its own takes the others, which are some instructions
+// more (8-bit moments of 134M elements in 476 us instead of 454 where all do).
+template <bool kFlush> __device__ __forceinline__ float sqrt_fast(float v) {
   float s;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(v));
+  if (kFlush) asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(v));
+  else asm("sqrt.approx.f32 %0, %1;" : "=f"(s) : "f"(v));
   return s;
 }
 
 // sqrt(v) after one of Newton's steps: within one place of the rounded root, and nearly always equal to it.  At zero
 // and infinity the step is NaN, which the minimum drops.
-__device__ __forceinline__ float sqrt_near(float v) {
-  const float s = sqrt_fast(v);
+template <bool kFlush> __device__ __forceinline__ float sqrt_near(float v) {
+  const float s = sqrt_fast<kFlush>(v);
   float r;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  if (kFlush) asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  else asm("rsqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
   return s + fminf(fmaf(-s, s, v) * (0.5f * r), s);
 }
 
@@ -245,7 +250,7 @@ struct Step {
 
 // A warp's blocks of one tensor: `block`, `block + stride`, ... below `end`.
 // P and G are the types of parameter and gradient where vectors are loaded; elsewhere the entry's are looked up.
-template <bool kVectors, bool kPacked, bool kMaster, typename P, typename G>
+template <bool kVectors, bool kPacked, bool kMaster, bool kFlush, typename P, typename G>
 __device__ __forceinline__ void update_blocks(const Entry& e, const Common& c, const Step& s, int block, int end, int stride) {
   const int lane = threadIdx.x & 31;
   using Weight = std::conditional_t<kMaster, float, P>;
@@ -288,7 +293,7 @@ __device__ __forceinline__ void update_blocks(const Entry& e, const Common& c, c
       m[i] = __fadd_rn(__fmul_rn(m[i], c.beta1), __fmul_rn(g[i], c.rest1));
       if (kPacked) v[i] = __fmul_rn(v[i], v[i]);
       v[i] = __fadd_rn(__fmul_rn(v[i], c.beta2), __fmul_rn(__fmul_rn(g[i], g[i]), c.rest2));
-      const float root = kPacked ? sqrt_near(v[i]) : sqrt_fast(v[i]);
+      const float root = kPacked ? sqrt_near<kFlush>(v[i]) : sqrt_fast<kFlush>(v[i]);
       p[i] = p[i] * s.decay - s.size * m[i] * reciprocal(fmaf(root, s.root_scale, c.eps));
       if (kPacked) v[i] = root;
     }
@@ -336,7 +341,7 @@ __device__ __forceinline__ void update_blocks(const Entry& e, const Common& c, c
 
 template <bool kPacked, bool kMaster, typename P, typename G>
 __device__ __forceinline__ void update_whole(const Entry& e, const Common& c, const Step& s, int block, int end, int stride) {
-  update_blocks<true, kPacked, kMaster, P, G>(e, c, s, block, end, stride);
+  update_blocks<true, kPacked, kMaster, true, P, G>(e, c, s, block, end, stride);
 }
 
 template <bool kPacked, bool kMaster, typename P>
@@ -346,11 +351,11 @@ __device__ __forceinline__ void update_whole(const Entry& e, const Common& c, co
   else update_whole<kPacked, kMaster, P, __half>(e, c, s, block, end, stride);
 }
 
-template <bool kPacked>
+template <bool kPacked, bool kFlush>
 __device__ __forceinline__ void update_tensor(const Entry& e, const Common& c, const Step& s, int block, int end, int stride) {
   // whole blocks by vectors where all of the tensor's pointers allow that; the last block may be cut
-  const int whole = e.vectors ? (int)min((long long)end, e.count / kBlock) : 0;
-  if (block < whole) {
+  const int whole = kFlush && e.vectors ? (int)min((long long)end, e.count / kBlock) : 0;
+  if (kFlush && block < whole) {
     if (e.param_type == FBFFTCONV_FLOAT32) update_whole<kPacked, false, float>(e, c, s, block, whole, stride);
     else if (e.param_type == FBFFTCONV_BFLOAT16 && e.master) update_whole<kPacked, true, __nv_bfloat16>(e, c, s, block, whole, stride);
     else if (e.param_type == FBFFTCONV_BFLOAT16) update_whole<kPacked, false, __nv_bfloat16>(e, c, s, block, whole, stride);
@@ -358,10 +363,10 @@ __device__ __forceinline__ void update_tensor(const Entry& e, const Common& c, c
     else update_whole<kPacked, false, __half>(e, c, s, block, whole, stride);
     block += (whole - block + stride - 1) / stride * stride;
   }
-  if (block < end) update_blocks<false, kPacked, false, float, float>(e, c, s, block, end, stride);
+  if (block < end) update_blocks<false, kPacked, false, kFlush, float, float>(e, c, s, block, end, stride);
 }
 
-template <int N>
+template <int N, bool kFlush>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<N> t) {
   __shared__ Step shared;
   const Common& c = t.c;
@@ -392,8 +397,8 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     k = lo;
     const Entry& e = t.entry[k];
     const int end = min(last, k + 1 < c.tensors ? t.entry[k + 1].first : c.blocks);
-    if (e.scale1) update_tensor<true>(e, c, s, b - e.first, end - e.first, stride);
-    else update_tensor<false>(e, c, s, b - e.first, end - e.first, stride);
+    if (e.scale1) update_tensor<true, kFlush>(e, c, s, b - e.first, end - e.first, stride);
+    else update_tensor<false, kFlush>(e, c, s, b - e.first, end - e.first, stride);
     b += (end - b + stride - 1) / stride * stride;
   }
   if (!c.advance) return;
@@ -407,9 +412,13 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
   }
 }
 
+// Whether a root that is flushed, one of v < 2^-126, can be more than 2^-20 of eps: it is divided by sqrt(1 - b2^t), at the
+// first step sqrt(1 - b2).  Such an optimizer goes by single elements: few are.
+bool small_eps(const fbfftconv_adamw_options& o) { return o.eps * sqrt(1 - o.beta2) < 0x1p-43; }
+
 int blocks_of(long long count) { return (int)((count + kBlock - 1) / kBlock); }
 
-template <int N>
+template <int N, bool kFlush>
 cudaError_t launch(const fbfftconv_adamw* h, const int* tensors, int count, const Common& common, cudaStream_t stream) {
   Table<N> table;
   table.c = common;
@@ -430,7 +439,7 @@ cudaError_t launch(const fbfftconv_adamw* h, const int* tensors, int count, cons
   static std::atomic<int> known{0};  // the same on every device of this architecture
   int resident = known.load(std::memory_order_relaxed);
   if (resident == 0) {
-    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, adamw_kernel<N>, kThreads, 0);
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, adamw_kernel<N, kFlush>, kThreads, 0);
     if (e != cudaSuccess) return e;
     known.store(resident, std::memory_order_relaxed);
   }
@@ -442,7 +451,13 @@ cudaError_t launch(const fbfftconv_adamw* h, const int* tensors, int count, cons
   const int grid = (int)(need < 1 ? 1 : need < most ? need : most);
   if (rounds == 1) table.c.run = (int)((blocks + (long long)grid * kWarps - 1) / ((long long)grid * kWarps));
   count_launch();
-  return launch_dependent(adamw_kernel<N>, dim3(grid), kThreads, 0, stream, table);
+  return launch_dependent(adamw_kernel<N, kFlush>, dim3(grid), kThreads, 0, stream, table);
+}
+
+template <int N>
+cudaError_t launch(const fbfftconv_adamw* h, const int* tensors, int count, const Common& common, cudaStream_t stream) {
+  return small_eps(h->options) ? launch<N, false>(h, tensors, count, common, stream)
+                               : launch<N, true>(h, tensors, count, common, stream);
 }
 
 int check_tensor(const fbfftconv_adamw_tensor& t, int i) {

@@ -388,3 +388,34 @@ def test_gradients_that_lie_in_what_is_stepped_are_refused():
     assert opt.grads[0] is g
     opt.step()
     assert opt.steps == 1
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-22, 1e-18, 1e-14, 1e-11])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_small_gradients_and_eps(eps, bits):
+    """Roots whose squares are below the normal numbers, where eps does not hide them.  A place of v is 2^-149 there: what
+    64 bits make of the moments that are left is off by that, twice with the product's, beside a step's usual 2^-19; v of
+    8-bit moments is the square of a root, which the codes round."""
+    sizes = [300, 1000, 7]
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    params = [torch.zeros(n, device="cuda") for n in sizes]
+    grads = [torch.empty(n, device="cuda").uniform_(1e-19, 4e-18, generator=gen) for n in sizes]
+    grads[0][::2] *= -1
+    opt = AdamW(params, grads, lr=1.0, betas=(0.9, 0.999), eps=eps, weightDecay=0.0, stateBits=bits, min8bitSize=1)
+    opt.step()
+    for p, g in zip(params, grads):
+        g = g.double()
+        v = 0.001 * g ** 2
+        off = 2.0 ** -148 / v  # of v, to its last place
+        root = (v / 0.001).sqrt()
+        want = -g / (root + eps)
+        assert ((p.double() - want).abs() <= (2.0 ** -19 + off) * want.abs()).all()
+    before, v = [p.double() for p in params], [_decode(opt, i, "r8") for i in range(3)]
+    m = [_decode(opt, i, "m8") for i in range(3)]
+    opt.step()
+    for p, g, x, m, v in zip(params, grads, before, m, v):
+        g, v = g.double(), v ** 2 if bits == 8 else v
+        m, v = 0.9 * m + 0.1 * g, 0.999 * v + 0.001 * g ** 2
+        root = (v / (1 - 0.999 ** 2)).sqrt()
+        want = x - m / (1 - 0.9 ** 2) / (root + eps)
+        assert ((p.double() - want).abs() <= (2.0 ** -18 + 3 * 2.0 ** -148 / v) * (want - x).abs() + 2.0 ** -22 * x.abs()).all()

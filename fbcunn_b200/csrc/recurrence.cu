@@ -889,7 +889,8 @@ int check_desc(const fbfftconv_recurrence_desc* d) {
   const int64_t strides[] = {d->x_stride, d->g_stride, d->z_stride, d->y_stride, d->grad_y_stride, d->grad_x_stride,
                              d->grad_g_stride, d->grad_z_stride};
   for (const int64_t s : strides)
-    if (s > (1ll << 26)) return op_fail(FBFFTCONV_ERR_UNSUPPORTED_SIZE, "more than 2^26 elements between rows");
+    if (s < 0) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "negative stride");
+    else if (s > (1ll << 26)) return op_fail(FBFFTCONV_ERR_UNSUPPORTED_SIZE, "more than 2^26 elements between rows");
   if (!known_type(d->type)) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "unknown element type");
   if (!d->offsets && ((d->length > 0 && d->sequences > d->rows / d->length) || d->rows != d->sequences * d->length))
     return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "rows are not sequences times length");

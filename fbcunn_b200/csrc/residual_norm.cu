@@ -652,6 +652,7 @@ int check_desc(const fbfftconv_norm_desc* d) {
   if (d->rows < 0 || d->channels <= 0) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "rows and channels must be positive");
   if (d->rows > kMostRows || d->u_stride > kMostStride || d->r_stride > kMostStride || d->gate_stride > kMostStride)
     return op_fail(FBFFTCONV_ERR_UNSUPPORTED_SIZE, "more than 2^30 rows, or elements between rows");
+  if (d->u_stride < 0 || d->r_stride < 0 || d->gate_stride < 0) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "negative stride");
   if (d->channels > kMostChannels) return op_fail(FBFFTCONV_ERR_UNSUPPORTED_SIZE, "more than %d channels", kMostChannels);
   if (!known_type(d->type) || !known_type(d->residual_type) ||
       (d->residual_type != d->type && d->residual_type != FBFFTCONV_FLOAT32))
@@ -693,7 +694,6 @@ int check_pointers(const Pointer (&all)[N], int device, int channels, int type, 
   for (const Pointer& q : all) {
     if (!q.p && q.needed) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "%s is null", q.name);
     if (!aligned_to(q.p, type_bytes(q.type))) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "%s is not aligned to its element", q.name);
-    if (q.needed && q.stride < 0) return op_fail(FBFFTCONV_ERR_INVALID_ARGUMENT, "%s has a negative stride", q.name);
     const int vector = type == FBFFTCONV_FLOAT32 ? 4 : 8;  // elements that travel together
     if (q.p && (!aligned_to(q.p, 16) || q.stride % vector)) *vectors = false;
   }

@@ -214,3 +214,15 @@ def test_the_limit_of_waits(lib):
     before = lib.fbfftconv_recurrence_wait_limit(5)
     assert before >= 100000 and lib.fbfftconv_recurrence_wait_limit(before) == 5
     assert lib.fbfftconv_recurrence_wait_limit(before) == before
+
+
+@pytest.mark.parametrize("field", ["x_stride", "g_stride", "z_stride", "y_stride", "grad_y_stride", "grad_x_stride", "grad_g_stride",
+                                   "grad_z_stride"])
+@pytest.mark.parametrize("stride", [-64, -(1 << 32) + 64, -(1 << 63)])
+def test_negative_strides(lib, field, stride):
+    """Also those that would be a sound one in 32 bits."""
+    d = ctypes.byref(_desc(**{field: stride}))
+    args = [4096 * (i + 1) for i in range(13)]
+    for rc in (lib.fbfftconv_recurrence(d, *args[:8], None),
+               lib.fbfftconv_recurrence_backward(d, *args, 1.0, 0, 4096, 1 << 20, None)):
+        assert rc == capi.ERR_INVALID_ARGUMENT and "negative stride" in capi.last_error()

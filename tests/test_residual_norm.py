@@ -47,3 +47,14 @@ def test_null_and_misaligned_pointers(lib):
     assert lib.fbfftconv_residual_norm(d, None, *[4096] * 9, None) == capi.ERR_INVALID_ARGUMENT  # a gate, but no block
     assert lib.fbfftconv_residual_norm(d, *[4096] * 9, 4100, None) == capi.ERR_INVALID_ARGUMENT  # stats
     assert lib.fbfftconv_residual_norm_backward(d, *[4096] * 16, float("nan"), 0, 4096, 1 << 20, None) == capi.ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("field", ["u_stride", "r_stride", "gate_stride"])
+@pytest.mark.parametrize("stride", [-1, -64, -(1 << 32) + 64, -(1 << 63)])
+def test_negative_strides(lib, field, stride):
+    """Also those that would be a sound one in 32 bits."""
+    d = ctypes.byref(_desc(**{field: stride}))
+    assert lib.fbfftconv_residual_norm(d, *[4096] * 10, None) == capi.ERR_INVALID_ARGUMENT
+    assert "negative stride" in capi.last_error()
+    assert lib.fbfftconv_residual_norm_backward(d, *[4096] * 16, 1.0, 0, 4096, 1 << 20, None) == capi.ERR_INVALID_ARGUMENT
+    assert "negative stride" in capi.last_error()

@@ -803,20 +803,22 @@ cudaLaunchConfig_t config_of(const Division& s, int cluster, size_t smem, cudaSt
   return config;
 }
 
-// Clusters of a size that the current GPU holds at once, asked once for each kernel.
+// Clusters of a size that the current GPU holds at once, asked once for each kernel and device.
+constexpr int kMostDevices = 64;     // of a process
+constexpr int kDividedKernels = 20;  // those below: two directions, five element layouts, with and without the output gate
 int resident_clusters(const void* kernel, int cluster, size_t smem) {
   struct Known {
     const void* kernel;
-    int device, clusters[kMostCluster + 1];
+    int16_t clusters[kMostCluster + 1];
   };
-  static Known known[64];
+  static Known known[kMostDevices][kDividedKernels];
   static std::mutex lock;
   const std::lock_guard<std::mutex> hold(lock);
   int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess) return 0;
-  Known* k = known;
-  while (k < known + 63 && k->kernel && (k->kernel != kernel || k->device != device)) ++k;
-  if (k->kernel != kernel || k->device != device) *k = Known{kernel, device, {}};
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMostDevices) return 0;
+  Known* k = known[device];
+  while (k < known[device] + kDividedKernels - 1 && k->kernel && k->kernel != kernel) ++k;
+  if (k->kernel != kernel) *k = Known{kernel, {}};
   if (k->clusters[cluster] == 0) {
     Division one{};
     one.tiles = one.segments = 1;
@@ -825,7 +827,7 @@ int resident_clusters(const void* kernel, int cluster, size_t smem) {
     int n = 0;
     cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);  // clusters of more than 8 blocks
     if (cudaOccupancyMaxActiveClusters(&n, kernel, &config) != cudaSuccess) cudaGetLastError(), n = 0;
-    k->clusters[cluster] = n > 0 ? n : -1;
+    k->clusters[cluster] = n > 0 ? (int16_t)n : -1;
   }
   return k->clusters[cluster];
 }
@@ -932,7 +934,6 @@ std::atomic<uint32_t> wait_polls{kPolls};
 
 // A word for each device, in host memory that its kernels write: what a call lost is known to the next one without a wait
 // for the device.  Null where there is none to be had.
-constexpr int kMostDevices = 256;
 int* wait_error_of(int device) {
   static std::atomic<int*> known{nullptr};
   static std::mutex lock;

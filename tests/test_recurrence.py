@@ -226,3 +226,13 @@ def test_negative_strides(lib, field, stride):
     for rc in (lib.fbfftconv_recurrence(d, *args[:8], None),
                lib.fbfftconv_recurrence_backward(d, *args, 1.0, 0, 4096, 1 << 20, None)):
         assert rc == capi.ERR_INVALID_ARGUMENT and "negative stride" in capi.last_error()
+
+
+def test_every_kernel_has_a_place_in_the_table_of_cluster_counts():
+    """On each device: a kernel without one would ask the driver at every call."""
+    with open(os.path.join(fb_build.CSRC, "recurrence.cu")) as f:
+        source = f.read()
+    layouts = re.search(r"#define BY_TYPE\(call\)(.*?)\n\n", source, re.S).group(1).count("call(")
+    kernels = len(re.findall(r"launch_divided\(\w+_kernel<T, V, \w+>", source)) * layouts
+    assert kernels == int(re.search(r"kDividedKernels = (\d+);", source).group(1))
+    assert re.search(r"known\[kMostDevices\]\[kDividedKernels\];", source)

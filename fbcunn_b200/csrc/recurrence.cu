@@ -60,7 +60,8 @@ struct RecArgs {
   int checkpoints_per_segment;
   int channels, wide_offsets, cluster;
   bool wide;             // rows begin on 16 bytes
-  uint32_t polls;        // of a wait for a cluster's stretches
+  uint32_t polls;        // of a wait for a cluster's stretches, after the first
+  uint32_t never;        // bytes that a wait is for and nobody sends: none, unless waits are to run out
   int* wait_error;       // set when one ran out: the device's word in host memory
 };
 
@@ -344,18 +345,19 @@ struct Exchange {
   int gave_up;
 };
 
-constexpr uint32_t kPolls = 1u << 20;  // of a microsecond each: about a second, where a round takes some microseconds
+constexpr uint32_t kPolls = 1u << 20;  // of a microsecond: about a second, where a round takes some microseconds
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-__device__ __forceinline__ bool wait_phase(uint32_t barrier, uint32_t parity, uint32_t polls) {
-  for (uint32_t i = 0; i < polls; ++i) {
-    uint32_t done;
+// Polls of a microsecond: one, and up to `more` of them.  (A loop that asks before its first poll cost 8 of 418 us
+// at 8 x 4096 x 2048 both ways, where there is no cluster at all.)
+__device__ __forceinline__ bool wait_phase(uint32_t barrier, uint32_t parity, uint32_t more) {
+  uint32_t done;
+  do {
     asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
                  : "=r"(done) : "r"(barrier), "r"(parity), "r"(1000u) : "memory");
-    if (done) return true;
-  }
-  return false;
+  } while (!done && more-- != 0);
+  return done;
 }
 
 template <int V>
@@ -387,7 +389,7 @@ __device__ __forceinline__ void send(uint32_t to, uint32_t barrier, int block, c
 // stretch goes to all blocks of the cluster with the bytes counted on their mbarriers: a cluster's barrier would have
 // waited for the outputs that are on their way to memory too.  A block sends a round's stretch after all of its warps
 // have read the round's before, so that nothing arrives in a buffer that is still read.  A block whose wait has run out
-// goes through its rounds without sending, counting or waiting any more, so that the others' waits run out in turn.
+// goes on as one without a cluster: it neither sends, counts nor waits any more, and the others' waits run out in turn.
 template <int V>
 __device__ __forceinline__ Vec<V> exchange(Exchange<V>& x, uint32_t round, int order, int rank, int blocks,
                                            const RecArgs& a, const Stretch<V>& mine, Vec<V>& carry) {
@@ -401,19 +403,18 @@ __device__ __forceinline__ Vec<V> exchange(Exchange<V>& x, uint32_t round, int o
   Stretch<V> all = join(before, mine);
 #pragma unroll 4
   for (int w = order + 1; w < kWarps; ++w) all = join(all, part[w][lane]);
-  if (blocks == 1) {
+  if (blocks == 1 || *reinterpret_cast<volatile int*>(&x.gave_up)) {
     const Vec<V> enter = apply(before, carry);
     carry = apply(all, carry);
     return enter;
   }
   const uint32_t barrier = shared_address(&x.arrived[half]);
-  const bool lost = *reinterpret_cast<volatile int*>(&x.gave_up);
-  if (threadIdx.x == 0 && !lost)
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"((uint32_t)(blocks * 32 * sizeof(Stretch<V>))) : "memory");
-  for (int k = lost ? blocks : order; k < blocks; k += kWarps) send(shared_address(&x.whole[half][rank][lane]), barrier, k, all);
-  if (!lost && !wait_phase(barrier, round / kTurns & 1, a.polls)) {
+  if (threadIdx.x == 0)
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"((uint32_t)(blocks * 32 * sizeof(Stretch<V>)) + a.never) : "memory");
+  for (int k = order; k < blocks; k += kWarps) send(shared_address(&x.whole[half][rank][lane]), barrier, k, all);
+  if (!wait_phase(barrier, round / kTurns & 1, a.polls)) {
     *reinterpret_cast<volatile int*>(&x.gave_up) = 1;
-    *reinterpret_cast<volatile int*>(a.wait_error) = 1;
+    asm volatile("st.global.u32 [%0], %1;" ::"l"(a.wait_error), "r"(1));
   }
 #pragma unroll 4
   for (int k = 0; k < rank; ++k) carry = apply(x.whole[half][k][lane], carry);
@@ -973,6 +974,7 @@ RecArgs common_args(const fbfftconv_recurrence_desc& d) {
   RecArgs a{};
   a.rows = (int)d.rows, a.length = (int)d.length, a.sequences = (int)d.sequences, a.channels = d.channels;
   a.offsets = d.offsets, a.wide_offsets = d.wide_offsets, a.polls = wait_polls.load(std::memory_order_relaxed);
+  a.never = a.polls ? 0 : 16;
   a.x_stride = or_dense(d.x_stride), a.g_stride = or_dense(d.g_stride), a.z_stride = or_dense(d.z_stride);
   a.y_stride = or_dense(d.y_stride), a.dy_stride = or_dense(d.grad_y_stride);
   a.dx_stride = or_dense(d.grad_x_stride), a.dg_stride = or_dense(d.grad_g_stride), a.dz_stride = or_dense(d.grad_z_stride);

@@ -406,7 +406,7 @@ int fbfftconv_recurrence_step(const fbfftconv_recurrence_desc* desc, const void*
 int fbfftconv_recurrence_status(int reset);
 int fbfftconv_recurrence_wait_selftest(fbfftconv_stream stream);
 /* The limit of those waits for the calls (and captures) from now on, in microseconds, about a second at first; returns
- * the one before.  0: a wait whose results are not there yet gives up at once. */
+ * the one before.  0, for tests: every wait runs out, after its first microsecond. */
 uint32_t fbfftconv_recurrence_wait_limit(uint32_t microseconds);
 
 /* ---- norms before and after a residual block ------------------------------------------------

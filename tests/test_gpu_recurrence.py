@@ -463,8 +463,8 @@ def test_other_shapes_while_another_stream_still_works():
 
 
 def test_waits_that_run_out_in_the_middle_of_a_call():
-    """With no time to wait, the blocks of a cluster go their ways, and the call ends: its results are lost, the status
-    says so, and the calls after it are as ever."""
+    """With waits that nothing ends, the blocks of a cluster go their ways, and the call ends: its results are lost, the
+    status says so, and the calls after it are as ever."""
     lib = capi.lib()
     made = [make((1, 3000), 1, 64, BF, seed=11), make((3000,), 2, 33, F32, seed=12)]
     offsets = [None, torch.tensor([0, 1100, 3000], dtype=torch.int32, device="cuda")]

@@ -725,9 +725,14 @@ cudaError_t forward(const NormArgs& a, const Shape& s, cudaStream_t stream) {
                           : launch_rows(norm_forward_kernel<T, TR, 16, 1024, false>, a, s, grid, 0, stream);
   const size_t stage = (size_t)s.threads * s.columns * (2 * sizeof(T) + sizeof(TR));
   if (s.columns == 8) return launch_rows(norm_forward_kernel<T, TR, 8, 256, true>, a, s, grid, stage, stream);
-  return s.threads <= 320   ? launch_rows(norm_forward_kernel<T, TR, 16, 320, true>, a, s, grid, stage, stream)
-         : s.threads <= 512 ? launch_rows(norm_forward_kernel<T, TR, 16, 512, true>, a, s, grid, stage, stream)
-                            : launch_rows(norm_forward_kernel<T, TR, 16, 1024, true>, a, s, grid, stage, stream);
+  // Above 256 threads an SM holds one block at the 118 registers of sixteen columns, but two of up to 320 threads at 96,
+  // which 16-bit values do with (16384 rows with a gate: 4352 wide 150 us instead of 207, 5120 wide 162 instead of 215).
+  // Up to 256 it holds two or more anyway, and 96 are only fewer (2560 wide 133 us instead of 108 with an fp32 stream,
+  // 4096 wide with a gate 137 instead of 129); fp32 spills more at 96 (5120 wide 288 us instead of 249).
+  if constexpr (sizeof(T) == 2)
+    if (s.threads > 256 && s.threads <= 320) return launch_rows(norm_forward_kernel<T, TR, 16, 320, true>, a, s, grid, stage, stream);
+  return s.threads <= 512 ? launch_rows(norm_forward_kernel<T, TR, 16, 512, true>, a, s, grid, stage, stream)
+                          : launch_rows(norm_forward_kernel<T, TR, 16, 1024, true>, a, s, grid, stage, stream);
 }
 
 template <typename T, typename TR, bool kAll>

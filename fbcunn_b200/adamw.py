@@ -30,6 +30,8 @@ class AdamW:
                    state(), adopted ones are the caller's to save
     seed           of the random rounding of 8-bit moments
 
+    lr, betas, eps, weightDecay and seed may be set anew between steps; they are those of all tensors: parameters that are
+    not to be decayed belong to an optimizer of their own, which is one launch more.
     Tensors are contiguous and on one GPU; gradients have their parameter's shape and any of the three types.
     A tensor whose storage has been replaced since the last step is noticed and used from then on, if it is still such
     a tensor of as many elements."""
@@ -111,6 +113,8 @@ class AdamW:
         if list(map(_address, self._watched)) != self._addresses or list(map(_nbytes, self._watched)) != self._sizes:
             self._check()
             self._rebuild()
+        elif self._built != (self.betas, self.eps, self.weightDecay, self.seed):
+            self._rebuild()
         capi.check(capi.lib().fbfftconv_adamw_step(
             self._handle, self.lr if lr is None else lr, gradScale, scalars, _stream(self.device)))
 
@@ -172,6 +176,7 @@ class AdamW:
                                                      ctypes.byref(handle)))
         self._destroy()
         self._handle = handle
+        self._built = (self.betas, self.eps, self.weightDecay, self.seed)
         self._watched = self.params + self.grads + [w for w in self.masters if w is not None]
         self._addresses, self._sizes = list(map(_address, self._watched)), list(map(_nbytes, self._watched))
 

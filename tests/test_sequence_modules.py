@@ -349,3 +349,19 @@ def test_the_state_has_the_masters_that_were_made_here(host):
     adopted.loadState(adopted.state())
     with pytest.raises(AssertionError):
         adopted.loadState(state)
+
+
+def test_hyperparameters_may_change_between_steps(host):
+    opt, *_ = optimizer()
+    opt.step()
+    made_once = sum(n == "fbfftconv_adamw_create" for n, _ in host.calls)
+    opt.step()
+    assert sum(n == "fbfftconv_adamw_create" for n, _ in host.calls) == made_once
+    for name, value, field in (("weightDecay", 0.5, "weight_decay"), ("eps", 1e-5, "eps"), ("seed", 9, "seed")):
+        setattr(opt, name, value)
+        opt.step()
+        assert getattr(host.last("fbfftconv_adamw_create")[2], field) == value
+    opt.betas = (0.5, 0.25)
+    opt.lr = 0.125
+    opt.step()
+    assert host.last("fbfftconv_adamw_create")[2].beta2 == 0.25 and host.last("fbfftconv_adamw_step")[1] == 0.125

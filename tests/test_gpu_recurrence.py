@@ -6,6 +6,10 @@ carries |g| u, exp and quotient a few u).  a + (1 - a) = 1 to u / 2, so an error
 as many rows as the memory reaches, N = min(length, 1 / min(1 - a)).  D sums |e| with weights a: S_t = |e_t| + a_{t+1}
 S_{t+1}, within S (6 u N + 4 eps).  Products add their factors' errors.  Below the normal numbers (|g| > 87) the smaller of a and 1 - a
 is good to 2^-126 alone (`lost`), which is added to eps times it there.  16-bit outputs add half a step."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -545,3 +549,29 @@ def test_one_module_in_several_layers():
     want = y.clone()
     check(m, [y, *table[1:]], dy, h0, dlast)
     assert torch.equal(y, want)
+
+
+FIRST_CALL = """
+import torch
+from fbcunn_b200 import GatedLinearRecurrence
+m = GatedLinearRecurrence(64)
+table = [torch.randn(1, 3000, 64, device="cuda") for _ in range(3)]
+dy = torch.randn(1, 3000, 64, device="cuda")
+graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+side.wait_stream(torch.cuda.current_stream())
+with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+    y = m.updateOutput(table)
+    grads = m.backward(table, dy)
+graph.replay()
+got = [t.clone() for t in (y, m.state, *grads, m.gradBias)]
+again = [m.updateOutput(table), m.state, *m.backward(table, dy), m.gradBias]
+assert all(torch.equal(a, b) for a, b in zip(got, again)) and m.status() == 0
+print("replayed")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    """What the library sets up at its first call is no part of a capture."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=240)
+    assert run.returncode == 0 and "replayed" in run.stdout, run.stderr[-2000:]

@@ -71,7 +71,8 @@ class GatedLinearRecurrence:
 
     def updateOutput(self, input, state=None, offsets=None):
         """state: the initial states, or None for zeros; offsets: int32 or int64, sequences + 1 on the device, for packed
-        rows, of which those outside of all sequences stay as they are in `output`."""
+        rows, of which those outside of all sequences stay as they are in `output` and the gradients: zero, or what an
+        earlier call of the same shapes left there."""
         x, g, z = self._prepare(input, offsets)
         self._check_state(state, "initial state")
         # what was returned before is an input now
@@ -194,7 +195,8 @@ class GatedLinearRecurrence:
                 self._graphs.append((self._output, self._state, self._checkpoints, self._grads, self._workspace, self._grad_state))
             self._captured = _capturing()
             self._workspace = self._grad_state = self._output = self._state = None
-            self._output = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            self._packed = offsets is not None
+            self._output = self._rows(x, self.channels)
             self._state = torch.empty((sequences, self.channels), dtype=torch.float32, device=x.device)
             self._checkpoints = self._grads = None
             self.checkpoints = None
@@ -209,12 +211,17 @@ class GatedLinearRecurrence:
                 f"the {what} is fp32 (sequences, channels)"
             assert state.device == self._where, "CUDA support only!"
 
+    def _rows(self, x, channels):
+        """A tensor of x's rows.  Packed ones outside of all sequences are never written: zeros, not what was in memory."""
+        make = torch.zeros if self._packed else torch.empty
+        return make(x.shape[:-1] + (channels,), dtype=x.dtype, device=x.device)
+
     def _another(self, t):
         """A tensor in the place of one that the module has given away."""
         if self._captured:
             self._graphs.append(t)
         self._made = self._made if _raw_stream(self._index) == self._made else -1  # of two streams: recorded on any
-        return torch.empty_like(t)
+        return self._rows(t, self.channels) if t is self._output else torch.empty_like(t)
 
     def _backward(self, input, gradOutput, scale, state, offsets, gradState, inputs, parameters):
         kept = self.checkpoints
@@ -226,7 +233,7 @@ class GatedLinearRecurrence:
         assert gradOutput.shape == x.shape and gradOutput.dtype == x.dtype, "gradOutput size mismatch"
         parts = 3 if self.outputGate else 2
         if self._grads is None:
-            self._projection = torch.empty(x.shape[:-1] + (parts * self.channels,), dtype=x.dtype, device=x.device)
+            self._projection = self._rows(x, parts * self.channels)
             n = int(capi.lib().fbfftconv_recurrence_workspace_bytes(self._desc_ref))
             self._workspace = torch.empty(max(n, 16), dtype=torch.uint8, device=x.device)
             self._grad_state = torch.empty_like(self._state)

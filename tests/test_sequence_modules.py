@@ -365,3 +365,16 @@ def test_hyperparameters_may_change_between_steps(host):
     opt.lr = 0.125
     opt.step()
     assert host.last("fbfftconv_adamw_create")[2].beta2 == 0.25 and host.last("fbfftconv_adamw_step")[1] == 0.125
+
+
+def test_packed_rows_that_no_sequence_has_are_zero(host, monkeypatch):
+    """In new outputs and gradients, and in those that take the place of given-away ones."""
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: empty(*a, **kw).fill_(77))
+    m, t = recurrent(), [made(9, 8) for _ in range(3)]
+    offsets = torch.tensor([0, 2, 5])
+    for _ in range(2):
+        y = m.updateOutput(t, offsets=offsets)
+        assert not y.any() and not any(g.any() for g in m.backward(t, t[0], offsets=offsets))
+        t[0] = y.as_subclass(OnDevice)
+    assert m.updateOutput(recurrence_table(2)).any()  # padded rows are all written

@@ -83,7 +83,6 @@ class GatedResidualNorm:
     def updateOutput(self, input):
         u, r, gate = self._prepare(input)
         stats = self._stats if self.train else None
-        self.stats = stats
         inputs = _ptr(u), r.data_ptr(), _ptr(gate)
         if self._r_at in inputs or self._v_at in inputs:
             self._give_away(inputs)
@@ -92,6 +91,7 @@ class GatedResidualNorm:
             self._v_at if self._v_at > 0 else None, _ptr(stats), _raw_stream(self._index))
         if status:
             capi.check(status)
+        self.stats = stats
         self.output = self._v if u is None else self._r_out if self._v is None else [self._r_out, self._v]
         return self.output
 

@@ -17,7 +17,7 @@ class Host:
     """Stands for the library and the stream: calls are (name, arguments), with descriptors and tables copied."""
 
     def __init__(self):
-        self.calls, self.stream, self.capturing, self.recorded = [], 0, False, []
+        self.calls, self.stream, self.capturing, self.recorded, self.refused = [], 0, False, [], ""
 
     def __getattr__(self, name):
         if not name.startswith("fbfftconv_"):
@@ -27,6 +27,10 @@ class Host:
             self.calls.append((name, [self._copy(a) for a in args]))
             if name.endswith("_bytes"):
                 return 64
+            if name == "fbfftconv_last_error":
+                return b"refused"
+            if name == self.refused:
+                return capi.ERR_INVALID_ARGUMENT
             if name == "fbfftconv_adamw_create":
                 args[3]._obj.value = 1
             return 0
@@ -378,3 +382,17 @@ def test_packed_rows_that_no_sequence_has_are_zero(host, monkeypatch):
         assert not y.any() and not any(g.any() for g in m.backward(t, t[0], offsets=offsets))
         t[0] = y.as_subclass(OnDevice)
     assert m.updateOutput(recurrence_table(2)).any()  # padded rows are all written
+
+
+@pytest.mark.parametrize("build,table,entry", [(recurrent, recurrence_table, "fbfftconv_recurrence"),
+                                               (norm, norm_table, "fbfftconv_residual_norm")])
+def test_no_backward_pass_of_a_refused_forward_pass(host, build, table, entry):
+    m, t = build(), table(2)
+    host.refused = entry
+    with pytest.raises(capi.FbfftconvError):
+        m.updateOutput(t)
+    with pytest.raises(AssertionError):
+        m.backward(t, t[0] if build is recurrent else t)
+    host.refused = ""
+    m.updateOutput(t)
+    m.backward(t, t[0] if build is recurrent else t)

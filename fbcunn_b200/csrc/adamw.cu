@@ -444,8 +444,9 @@ cudaError_t launch(const fbfftconv_adamw* h, const int* tensors, int count, cons
     known.store(resident, std::memory_order_relaxed);
   }
   // 32-bit moments: many short-lived blocks, which keep the warps within one stretch of each tensor (134M elements in
-  // 562 us at 16 rounds of blocks, 607 at 4, 681 at 1).  8-bit moments are bound by the instructions, a block's start
-  // among them: one round (482 us, 500 at 4, 550 at 16).
+  // 560 us at 16 rounds of blocks, 591 at 4, 677 at 1).  8-bit moments are bound by the instructions, a warp's start in a
+  // tensor among them: one round, and a warp's blocks in a row (134M elements in 40 tensors 459 us, every so many-th at 4
+  // rounds 490; 11M in 60 tensors 37 and 47; in one tensor, which has few starts, 134M take 425 and 414).
   const int rounds = 2 * packed_blocks > blocks ? 1 : 16;
   const long long most = (long long)sm_count() * resident * rounds, need = (blocks + kWarps - 1) / kWarps;
   const int grid = (int)(need < 1 ? 1 : need < most ? need : most);

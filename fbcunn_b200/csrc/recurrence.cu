@@ -11,8 +11,8 @@
 // (distributed shared memory) and, from one round of rows to the next, in registers: one pass over memory, in an order
 // that only the sizes decide.  The rows of the next round are under way (cp.async, by the thread that will use them)
 // while this one is computed.  Bytes would allow 8 x 4096 x 2048 bf16 both ways in 226 us; it takes 418, bound by issue
-// and latency: 40 to 46 instructions an element forward, 83 backward, with 128 registers and so 16 warps an SM.  1 - a is formed first where a is the larger, so that a + (1 - a) = 1 to the last place and long memories
-// do not drift.
+// and latency: 40 to 46 instructions an element forward, 83 backward, with 128 registers and so 16 warps an SM.  1 - a is
+// formed first where a is the larger, so that a + (1 - a) = 1 to the last place and long memories do not drift.
 #include <cooperative_groups.h>
 #include <math.h>
 #include <string.h>
@@ -272,8 +272,9 @@ template <typename T, int V> __device__ __forceinline__ void store_word(T* p, Ve
 // The words of a warp's next rows: in shared memory, on their way there while this round is computed.  A slot holds
 // one tensor's rows, 128 bytes each; it is filled anew as soon as the round has read it, one group of copies after the
 // scan and one after the outputs, so that the oldest group but one is always the one that is waited for.  Where rows
-// begin on 16 bytes a lane copies such pieces of its warp's rows, past the L1 cache (`wide`; 8 x 4096 x 1024 bf16 takes 83
-// and 154 us forward and backward, 1026 channels, whose rows begin on 4 bytes, 114 and 179); else each its own words.  Single 16-bit values, which cp.async does not copy, are loaded where they are read.
+// begin on 16 bytes a lane copies such pieces of its warp's rows, past the L1 cache (`wide`; 8 x 4096 x 1024 bf16 takes 84
+// and 153 us forward and backward, 1026 channels, whose rows begin on 4 bytes, 115 and 176); else each its own words.
+// Single 16-bit values, which cp.async does not copy, are loaded where they are read (1025 channels: 127 and 261).
 template <typename T, int V, int kRows>
 struct Words {
   static constexpr bool kAsync = sizeof(T) * V == 4;
@@ -833,10 +834,10 @@ int resident_clusters(const void* kernel, int cluster, size_t smem) {
   return k->clusters[cluster];
 }
 
-// The widest cluster of which the GPU holds as many at once as there are: a second wave of them would double the time
-// (16 clusters of 16 blocks, of which 14 are held, for 131072 x 1024: 1214 us where those of 13 took 690).  Narrower
-// ones are slower, a round takes as long with fewer rows (of 8, 9 and 11 blocks: 725, 650 and 571 us where those of 13
-// took 489).  A block has at least one round of rows.
+// The widest cluster of which the GPU holds as many at once as there are: those that are left would begin when the others
+// have ended (131072 x 1024 f16 forward by 16 clusters: of 16 blocks, of which 14 are held, 545 us, of 13 blocks 420).
+// Narrower ones are slower, a round takes as long with fewer rows (8, 9, 11 and 12 blocks: 620, 556, 490 and 452 us).  A
+// block has at least one round of rows.
 template <typename K>
 cudaError_t launch_divided(K kernel, RecArgs a, const Division& s, int tile_rows, size_t smem, int* parts, cudaStream_t stream) {
   const void* const pointer = reinterpret_cast<const void*>(kernel);

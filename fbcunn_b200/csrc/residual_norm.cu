@@ -8,10 +8,10 @@
 //   dw2 = sum dv hat2, db2 = sum dv, dw1 = sum dn hat1, db1 = sum dn;  dg summed over the rows that share a gate row
 //
 // A row is held in the registers of one warp or one block between its sums, so each tensor moves once; 16384 x 4096 bf16
-// with a gate per token takes 421 us both ways where its bytes would take 266, bound by the latency of a row's sums and
-// by issue (43 and 92 instructions an element).  Sums over a row go by shuffles and one exchange through shared memory; a layer norm's deviation is
-// taken about the mean, in a sum of its own.  Sums over rows stay in registers while a block walks its rows, and a
-// second kernel adds the blocks' sums in a fixed order: the same call gives the same bits.
+// with a gate per token takes 413 us both ways where its bytes would take 266, bound by the latency of a row's sums and
+// by issue (38 and 92 instructions an element).  Sums over a row go by shuffles and one exchange through shared memory; a
+// layer norm's deviation is taken about the mean, in a sum of its own.  Sums over rows stay in registers while a block
+// walks its rows, and a second kernel adds the blocks' sums in a fixed order: the same call gives the same bits.
 #include <math.h>
 
 #include <type_traits>
@@ -627,9 +627,11 @@ struct Shape {
 };
 
 // Short rows share a block, a warp each; a longer row has a block to itself, whose lanes meet at its barriers.  Rows of
-// whole vectors go through the ring (8192 x 7000 f16 with a gate: 152 and 347 us forward and backward; 7001 without:
-// 483 and 1109) where one row of every tensor fits shared memory.  Sixteen columns a thread are more than the registers
-// hold with the sums over rows: eight, until a row is wider than 512 threads (4096: 663 us both ways against 675).
+// whole vectors go through the ring (8192 x 7000 f16 with a gate: 150 and 351 us forward and backward; 7001, without the
+// ring: 475 and 1112) where one row of every tensor fits shared memory.  Sixteen columns a thread are more than the
+// registers hold with the sums over rows: eight in the backward pass (16384 x 4096 with a gate 285 us, sixteen 319), until
+// a row is wider than 512 threads; from there on it spills.  Forward, eight keep more blocks on an SM until a row is wider
+// than 256 threads (16384 x 2048 bf16 57 us, sixteen 59).
 Shape shape_of(int channels, int columns, bool ring) {
   const int lanes = (channels + 32 * columns - 1) / (32 * columns) * 32;
   return {lanes, lanes == 32 ? 128 : lanes, columns, ring};
@@ -716,8 +718,10 @@ cudaError_t launch_rows(K kernel, NormArgs a, const Shape& s, int grid, size_t s
 template <typename T, typename TR>
 cudaError_t forward(const NormArgs& a, const Shape& s, cudaStream_t stream) {
   const long long slots = s.threads / s.lanes, need = (a.rows + slots - 1) / slots;
-  // a thousand threads an SM, in blocks that walk several rows each (24 x 513 x 1000 f32 both ways: 125 us, with eight
-  // blocks an SM whatever their size 131; 131072 x 256 bf16 forward 61 and 71, 8192 x 5120 113 and 115)
+  // Blocks that walk several rows each: four an SM from 256 threads up, 1024 threads an SM below.  Those are one or more
+  // full sets of what an SM holds; other numbers leave a set half empty (8192 x 5120 bf16 with an fp32 stream 112 us, five
+  // an SM 130, seven 124), fewer threads leave loads too few (131072 x 256 bf16 50 us, half as many 62, 12312 x 1000 f32 42
+  // and 57), and more are more starts (8192 x 8192 bf16 122 us, eight an SM 126, sixteen 137).
   const long long most = (long long)sm_count() * (s.threads >= 256 ? 4 : 1024 / s.threads);
   const int grid = (int)(need < most ? need : most);
   if (!s.ring)

@@ -361,13 +361,13 @@ int fbfftconv_adamw_step(fbfftconv_adamw* h, double lr, float grad_scale, const 
 /* ---- gated linear recurrence along sequences -------------------------------------------------
  *   a_t = sigmoid(g_t + bias),  h_t = a_t h_{t-1} + (1 - a_t) x_t,  y_t = h_t silu(z_t)   (y_t = h_t where z is null)
  * with h_{-1} the sequence's initial state (zero where state0 is null).  x, g, z, y are rows of `channels` neighbours of
- * one type, their stride (elements, at most 2^26; 0 = channels) apart; bias (channels), states (sequences, channels) and checkpoints
- * are fp32.  The rows are those of `sequences` sequences of `length` rows one behind the other (rows = sequences *
+ * one type, their stride (elements, at most 2^26; 0 = channels) apart; bias (channels), states (sequences, channels) and
+ * checkpoints are fp32.  The rows are those of `sequences` sequences of `length` rows one behind the other (rows = sequences *
  * length), or, with offsets (sequences + 1 integers on the device, 32 or with wide_offsets 64 bits wide, not falling),
  * sequence i has rows [offsets[i], offsets[i + 1]) of `rows`; rows outside of all sequences are neither read nor
- * written.  Sequences may be empty: their state passes through.  At most
- * 2^30 rows and sequences.  Nothing of a sequence, not even a NaN, reaches the
- * next.  Results do not depend on the timing of blocks: the same call gives the same bits. */
+ * written.  Sequences may be empty: their state passes through.  At most 2^30 rows and sequences.  Nothing of a sequence,
+ * not even a NaN, reaches the next.  Results do not depend on the timing of blocks: the same call gives the same bits.
+ * What a call writes shares no memory with what it reads. */
 typedef struct fbfftconv_recurrence_desc {
   int64_t rows, sequences, length;
   const void* offsets;             /* or null */
@@ -419,7 +419,8 @@ uint32_t fbfftconv_recurrence_wait_limit(uint32_t microseconds);
  * gate_rows rows, a divisor of rows: consecutive rows / gate_rows rows share one (a gate for each token, sequence, or
  * for all).  u may be null when neither post-norm nor gate is there: v = pre(r), and r' is r itself, neither scaled nor
  * written.  Weights and biases are fp32 (channels); a bias may be null.  channels <= 16384, rows and strides <= 2^30.
- * Rows of u, r and the gate lie their stride (elements; 0 = channels) apart, everything else is contiguous. */
+ * Rows of u, r and the gate lie their stride (elements; 0 = channels) apart, everything else is contiguous.  What a call
+ * writes shares no memory with what it reads. */
 enum { FBFFTCONV_NORM_NONE = 0, FBFFTCONV_NORM_RMS = 1, FBFFTCONV_NORM_LAYER = 2 };
 enum { FBFFTCONV_GATE_NONE = 0, FBFFTCONV_GATE_LINEAR = 1, FBFFTCONV_GATE_SIGMOID = 2 };
 typedef struct fbfftconv_norm_desc {

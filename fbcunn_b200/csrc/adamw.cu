@@ -218,8 +218,8 @@ __device__ __forceinline__ float magnitude(const float (&x)[8]) {
 }
 
 // Flushed, what is below the smallest normal number counts as zero: a root that is then below 2^-63 is nothing beside eps,
-// unless eps is nearly as small (`small_eps`): then a kernel of its own takes the others, which are some instructions
-// more (8-bit moments of 134M elements in 476 us instead of 454 where all do).
+// unless eps is nearly as small (`small_eps`): a kernel of its own takes the others then, which are some instructions more
+// (134M elements in one tensor with masters and 8-bit moments 434 us and 459; 32-bit moments take as long).
 template <bool kFlush> __device__ __forceinline__ float sqrt_fast(float v) {
   float s;
   if (kFlush) asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(v));
@@ -339,28 +339,28 @@ __device__ __forceinline__ void update_blocks(const Entry& e, const Common& c, c
   }
 }
 
-template <bool kPacked, bool kMaster, typename P, typename G>
+template <bool kPacked, bool kMaster, bool kFlush, typename P, typename G>
 __device__ __forceinline__ void update_whole(const Entry& e, const Common& c, const Step& s, int block, int end, int stride) {
-  update_blocks<true, kPacked, kMaster, true, P, G>(e, c, s, block, end, stride);
+  update_blocks<true, kPacked, kMaster, kFlush, P, G>(e, c, s, block, end, stride);
 }
 
-template <bool kPacked, bool kMaster, typename P>
+template <bool kPacked, bool kMaster, bool kFlush, typename P>
 __device__ __forceinline__ void update_whole(const Entry& e, const Common& c, const Step& s, int block, int end, int stride) {
-  if (e.grad_type == FBFFTCONV_FLOAT32) update_whole<kPacked, kMaster, P, float>(e, c, s, block, end, stride);
-  else if (e.grad_type == FBFFTCONV_BFLOAT16) update_whole<kPacked, kMaster, P, __nv_bfloat16>(e, c, s, block, end, stride);
-  else update_whole<kPacked, kMaster, P, __half>(e, c, s, block, end, stride);
+  if (e.grad_type == FBFFTCONV_FLOAT32) update_whole<kPacked, kMaster, kFlush, P, float>(e, c, s, block, end, stride);
+  else if (e.grad_type == FBFFTCONV_BFLOAT16) update_whole<kPacked, kMaster, kFlush, P, __nv_bfloat16>(e, c, s, block, end, stride);
+  else update_whole<kPacked, kMaster, kFlush, P, __half>(e, c, s, block, end, stride);
 }
 
 template <bool kPacked, bool kFlush>
 __device__ __forceinline__ void update_tensor(const Entry& e, const Common& c, const Step& s, int block, int end, int stride) {
   // whole blocks by vectors where all of the tensor's pointers allow that; the last block may be cut
-  const int whole = kFlush && e.vectors ? (int)min((long long)end, e.count / kBlock) : 0;
-  if (kFlush && block < whole) {
-    if (e.param_type == FBFFTCONV_FLOAT32) update_whole<kPacked, false, float>(e, c, s, block, whole, stride);
-    else if (e.param_type == FBFFTCONV_BFLOAT16 && e.master) update_whole<kPacked, true, __nv_bfloat16>(e, c, s, block, whole, stride);
-    else if (e.param_type == FBFFTCONV_BFLOAT16) update_whole<kPacked, false, __nv_bfloat16>(e, c, s, block, whole, stride);
-    else if (e.master) update_whole<kPacked, true, __half>(e, c, s, block, whole, stride);
-    else update_whole<kPacked, false, __half>(e, c, s, block, whole, stride);
+  const int whole = e.vectors ? (int)min((long long)end, e.count / kBlock) : 0;
+  if (block < whole) {
+    if (e.param_type == FBFFTCONV_FLOAT32) update_whole<kPacked, false, kFlush, float>(e, c, s, block, whole, stride);
+    else if (e.param_type == FBFFTCONV_BFLOAT16 && e.master) update_whole<kPacked, true, kFlush, __nv_bfloat16>(e, c, s, block, whole, stride);
+    else if (e.param_type == FBFFTCONV_BFLOAT16) update_whole<kPacked, false, kFlush, __nv_bfloat16>(e, c, s, block, whole, stride);
+    else if (e.master) update_whole<kPacked, true, kFlush, __half>(e, c, s, block, whole, stride);
+    else update_whole<kPacked, false, kFlush, __half>(e, c, s, block, whole, stride);
     block += (whole - block + stride - 1) / stride * stride;
   }
   if (block < end) update_blocks<false, kPacked, false, kFlush, float, float>(e, c, s, block, end, stride);
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
 }
 
 // Whether a root that is flushed, one of v < 2^-126, can be more than 2^-20 of eps: it is divided by sqrt(1 - b2^t), at the
-// first step sqrt(1 - b2).  Such an optimizer goes by single elements: few are.
+// first step sqrt(1 - b2).
 bool small_eps(const fbfftconv_adamw_options& o) { return o.eps * sqrt(1 - o.beta2) < 0x1p-43; }
 
 int blocks_of(long long count) { return (int)((count + kBlock - 1) / kBlock); }

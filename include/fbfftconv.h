@@ -325,7 +325,7 @@ enum { FBFFTCONV_FLOAT32 = 0, FBFFTCONV_BFLOAT16 = 1, FBFFTCONV_FLOAT16 = 2 };
  * ceil(count / 256) blocks each).  Codes are rounded up or down at random in proportion to what is cut off, by a hash
  * of seed, step, the tensor's place in the list and the element's in the tensor: the same call gives the same codes.
  * A gradient that is not finite leaves its block without finite moments.  Moments are fp32 numbers: v is lost where
- * (1 - beta2) g^2 is below them, from |g| of some 1e-21 down, and an eps below some 1e-12 takes a slower path.
+ * (1 - beta2) g^2 is below them, from |g| of some 1e-21 down.
  *
  * `master`, for 16-bit parameters, is the weight itself in fp32; param is then its rounded copy and is only written.
  * Every array is contiguous and aligned to its element; 16-byte alignment (8 for codes) is what the vector loads want.
